@@ -249,6 +249,106 @@ MRN_API void mrn_group_destroy(mrn_group* group);
 MRN_API int mrn_evaluate_device_static(mrn_ctx* ctx, int n, const uint8_t* d_boards, const int32_t* d_legal,
                                        float* d_priors, float* d_wdl, void* stream);
 
+/* ---- policy operators ------------------------------------------------------------------
+ *
+ * Three operators between move lists and a move: slot rows built from the lengths of the lists,
+ * logits under penalties, biases and masks (with their priors), and the choice of one action per
+ * row. They need nothing of a context but its device, its error message and its status word, and
+ * keep nothing: no workspace, no state from one call to the next. Rows are positions, or any other
+ * requests; the columns of a row are the actions 0, 1, ... in order or slots that name an action
+ * each, and need not have the sizes of the network.
+ *
+ * Every pointer is to memory that the context's device can read and, for outputs, write, aligned to
+ * its elements. The work is enqueued on `stream` without synchronising (a cudaStream_t of the
+ * context's device; NULL = the context's own stream; the legacy default stream is the handle 1,
+ * cudaStreamLegacy) and may be captured into a graph. The caller's current device is left as it
+ * was. Nothing orders these calls with work on other streams, the context's passes included: that
+ * is the caller's, with events. Outputs must not overlap inputs or one another, except where it
+ * says so. Numbers on the device cannot be refused by the call: what a bad one does is said with
+ * the argument, and none of them makes a kernel read or write outside the buffers. */
+
+/* Element type of logits. */
+typedef enum mrn_type {
+  MRN_TYPE_F32 = 0,
+  MRN_TYPE_F16 = 1,
+  MRN_TYPE_BF16 = 2,
+} mrn_type;
+
+/* Columns a row of the policy operators may have. */
+#define MRN_MAX_WIDTH (1 << 18)
+
+/* What changes the logits of a batch of rows. Strides count elements between rows; a stride of 0
+ * makes every row share one list. Unused parts are NULL (or have length 0).
+ *
+ * With c = how often the history of the row holds the column's action, a column's logit x becomes,
+ * in f32, each operation rounded once and in this order,
+ *   1. if c > 0: x = x > 0 ? x / repetition : x * repetition; x = (x - frequency * c) - presence;
+ *   2. for each entry of the bias list that names the action, in the list's order: x = x + value;
+ *   3. -inf if the mask does not allow the action or the slot is empty (whatever the logit held,
+ *      NaN included). */
+typedef struct mrn_rules {
+  int32_t actions;             /* ids lie in [0, actions); without `columns`, at least the width */
+  const int32_t* columns;      /* [rows, width]: the action of each slot, negative where it is empty; an
+                                  id >= actions counts as empty and sets the status word, as in
+                                  mrn_evaluate_device. NULL: column c is action c */
+  int64_t columns_stride;
+  const uint32_t* mask;        /* [rows, ceil(actions / 32)]: action a is allowed where bit a % 32 of word
+                                  a / 32 is set */
+  int64_t mask_stride;
+  const int32_t* bias_actions; /* [rows, bias_len]; ids outside [0, actions) change nothing */
+  const float* bias_values;    /* [rows, bias_len] */
+  int32_t bias_len;
+  int64_t bias_stride;
+  const int32_t* history;      /* [rows, history_len]; ids outside [0, actions) change nothing */
+  const int32_t* history_lens; /* [rows]: entries of each row's history that count, clamped to
+                                  [0, history_len]; NULL: all of them */
+  int32_t history_len;
+  int64_t history_stride;
+  const float* repetition;     /* [rows], positive; NULL: 1 */
+  const float* presence;       /* [rows]; NULL: 0 */
+  const float* frequency;      /* [rows]; NULL: 0 */
+} mrn_rules;
+
+/* Lays `rows` lists, stored one behind the other in `entries`, out in slot rows of `width`:
+ *   starts[r] = lengths[0] + ... + lengths[r - 1], r = 0 .. rows;
+ *   table[r * width + s] = entries[starts[r] + s] for s < lengths[r], and -1 behind the list;
+ *   map[starts[r] + s] = r * width + s, the slot of each entry.
+ * With width = MRN_MAX_LEGAL the table is the `legal` argument of mrn_evaluate_device. `count` is the
+ * number of entries in `entries` and in `map`; where the lists are longer together, the entries
+ * behind `count` are -1 in the table, and where they are shorter, the rest of `map` is left as it
+ * was. Lengths outside [0, width] are clamped. Lists longer than `count` and clamped lengths set the status
+ * word. `map` may be NULL. rows * width is at most 2^31 - 1. */
+MRN_API int mrn_slot_table(mrn_ctx* ctx, int rows, int width, const int32_t* lengths, int count, const int32_t* entries,
+                           int32_t* starts, int32_t* table, int32_t* map, void* stream);
+
+/* The rows' logits under `rules` (NULL: none), rounded to `type` into `out`, and their softmax at
+ * each row's temperature (NULL: 1) into `priors`, f32; either output may be NULL. `out` may be the
+ * logits themselves (the same pointer and stride). A masked column's prior is 0; a row that
+ * nothing is left of has priors of 0. At a temperature of 0 or below, the largest logit has the
+ * prior 1 (the lowest column of several). Where the largest logit is +inf, the columns that hold
+ * it share the row. A NaN that is left in a row, or as its temperature, makes the priors of its
+ * columns that are left NaN. */
+MRN_API int mrn_adjust_logits(mrn_ctx* ctx, int rows, int width, const void* logits, int type, int64_t stride,
+                              const mrn_rules* rules, const float* temperature, void* out, int64_t out_stride,
+                              float* priors, int64_t priors_stride, void* stream);
+
+/* One column per row, drawn from the logits under `rules` at the row's temperature. With the columns
+ * in the order of their adjusted logits, largest first and the lower column first among equals, the
+ * row keeps the first top_k[row] of them (all, if that is <= 0) and of those the shortest run, at
+ * least one, whose share of their mass is top_p[row] or more (all, if that is 1 or more or NaN). The
+ * column drawn is the lowest one up to which the kept mass, in column order, is more than
+ * uniform[row] of the whole. At a temperature of 0 or below it is the largest logit's, and so it is
+ * without `uniform`. Weights are whole multiples of 2^-40 of the largest.
+ *   column[row]: the column, or -1 where nothing is left of the row, or a NaN is;
+ *   action[row]: its action (NULL: not wanted);
+ *   prob[row]: its share of the kept mass, 1 at a temperature of 0; 0 where nothing is left, NaN
+ *   where a NaN is (NULL: not wanted).
+ * top_k, top_p, uniform and temperature are [rows] each, or NULL. */
+MRN_API int mrn_choose_actions(mrn_ctx* ctx, int rows, int width, const void* logits, int type, int64_t stride,
+                               const mrn_rules* rules, const float* temperature, const int32_t* top_k,
+                               const float* top_p, const float* uniform, int32_t* column, int32_t* action, float* prob,
+                               void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -52,6 +52,13 @@ MRN_TEST_API int mrn_test_attention(const void* qkv, void* out, int positions, i
 MRN_TEST_API int mrn_test_layernorm(const void* x, const float* gamma, const float* beta, float eps, int e4m3,
                                     float inv_q, void* out, int rows, int d, void* stream);
 
+/* A context of `device` with no network, stream or device memory (no device is touched), for the
+ * checks of the policy operators' arguments: this library also holds mrn_slot_table,
+ * mrn_adjust_logits and mrn_choose_actions. */
+MRN_TEST_API void* mrn_test_context(int device);
+MRN_TEST_API const char* mrn_test_context_error(void* ctx);
+MRN_TEST_API void mrn_test_context_free(void* ctx);
+
 MRN_TEST_API const char* mrn_test_last_error(void);
 
 #ifdef __cplusplus

@@ -9,7 +9,7 @@ caller never silently runs anything but the CUDA path.
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_uint8, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_uint8, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libmarina_b200.so"
@@ -28,6 +28,10 @@ PRECISION_FP8_X2 = 3
 PRECISIONS = {"bf16": PRECISION_BF16, "fp8w": PRECISION_FP8_WEIGHTS, "fp8": PRECISION_FP8,
               "fp8x2": PRECISION_FP8_X2}
 
+# Element types of the policy operators' logits.
+TYPES = {"f32": 0, "f16": 1, "bf16": 2}
+MAX_WIDTH = 1 << 18
+
 PROFILE_SLOTS = ("embed", "layernorm", "gemm", "attention", "heads")
 
 # Every symbol each header declares; `tests/test_abi.py` checks the libraries export exactly these.
@@ -37,9 +41,10 @@ EXPORTS = (
     "mrn_group_create", "mrn_group_evaluate", "mrn_group_size", "mrn_group_context", "mrn_group_describe",
     "mrn_group_last_error", "mrn_group_destroy",
     "mrn_evaluate_device_static",
+    "mrn_slot_table", "mrn_adjust_logits", "mrn_choose_actions",
 )
 TEST_EXPORTS = ("mrn_test_gemm", "mrn_test_gemm_wait_expiry", "mrn_test_attention", "mrn_test_layernorm",
-                "mrn_test_last_error")
+                "mrn_test_context", "mrn_test_context_error", "mrn_test_context_free", "mrn_test_last_error")
 
 
 class MrnLinear(ctypes.Structure):
@@ -69,6 +74,14 @@ class MrnArch(ctypes.Structure):
                 ("square_token_start", c_int32), ("fp8_amax", POINTER(c_float))]
 
 
+class MrnRules(ctypes.Structure):
+    _fields_ = [("actions", c_int32), ("columns", c_void_p), ("columns_stride", c_int64), ("mask", c_void_p),
+                ("mask_stride", c_int64), ("bias_actions", c_void_p), ("bias_values", c_void_p), ("bias_len", c_int32),
+                ("bias_stride", c_int64), ("history", c_void_p), ("history_lens", c_void_p), ("history_len", c_int32),
+                ("history_stride", c_int64), ("repetition", c_void_p), ("presence", c_void_p),
+                ("frequency", c_void_p)]
+
+
 _lib = None
 _test_lib = None
 
@@ -86,6 +99,11 @@ SIGNATURES = {
     "mrn_describe": (c_char_p, [c_void_p]),
     "mrn_last_error": (c_char_p, [c_void_p]),
     "mrn_destroy": (None, [c_void_p]),
+    "mrn_slot_table": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "mrn_adjust_logits": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int, c_int64, POINTER(MrnRules), c_void_p,
+                                  c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
+    "mrn_choose_actions": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int, c_int64, POINTER(MrnRules), c_void_p,
+                                   c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "mrn_group_create": (c_int, [POINTER(MrnArch), POINTER(MrnWeights), POINTER(c_int), c_int, c_int, c_int,
                                  POINTER(c_void_p)]),
     "mrn_group_evaluate": (c_int, [c_void_p, c_int, POINTER(c_uint8), POINTER(c_int32), POINTER(c_float),
@@ -105,7 +123,11 @@ TEST_SIGNATURES = {
     "mrn_test_attention": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p]),
     "mrn_test_layernorm": (c_int, [c_void_p, c_void_p, c_void_p, c_float, c_int, c_float, c_void_p, c_int, c_int,
                                    c_void_p]),
+    "mrn_test_context": (c_void_p, [c_int]),
+    "mrn_test_context_error": (c_char_p, [c_void_p]),
+    "mrn_test_context_free": (None, [c_void_p]),
     "mrn_test_last_error": (c_char_p, []),
+    **{name: SIGNATURES[name] for name in ("mrn_slot_table", "mrn_adjust_logits", "mrn_choose_actions")},
 }
 
 

@@ -10,6 +10,7 @@
 #include "../../include/marina_b200_test.h"
 #include "gemm.h"
 #include "kernels.cuh"
+#include "runtime.h"
 
 namespace {
 thread_local char g_test_error[512];
@@ -147,5 +148,15 @@ MRN_TEST_API int mrn_test_layernorm(const void* x, const float* gamma, const flo
   }
   return MRN_OK;
 }
+
+MRN_TEST_API void* mrn_test_context(int device) {
+  mrn_ctx* c = new mrn_ctx();
+  c->device = device;
+  return c;
+}
+
+MRN_TEST_API const char* mrn_test_context_error(void* ctx) { return static_cast<mrn_ctx*>(ctx)->last_error.c_str(); }
+
+MRN_TEST_API void mrn_test_context_free(void* ctx) { delete static_cast<mrn_ctx*>(ctx); }
 
 }  // extern "C"

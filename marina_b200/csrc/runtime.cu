@@ -18,6 +18,7 @@
 #include "gemm.h"
 #include "kernels.cuh"
 #include "launch.h"
+#include "policy.cuh"
 #include "runtime.h"
 
 namespace {
@@ -493,6 +494,8 @@ bool is_pinned(const void* p) {
 int check_status(mrn_ctx* c, int word) {
   if (word == 0) return MRN_OK;
   if (word == mrn::kErrBadAction) return c->fail(MRN_ERR_ACTION, "a legal slot held an action index >= %d", MRN_ACTIONS);
+  if (word == mrn::kErrBadLength)
+    return c->fail(MRN_ERR_ARGUMENT, "a slot table's list length was outside [0, width], or its lists longer than the entries");
   return c->fail(MRN_ERR_DEVICE_FAULT, "device-side wait gave up in a GEMM (code %d)", word);
 }
 
@@ -588,6 +591,7 @@ MRN_API int mrn_create(const mrn_arch* arch, const mrn_weights* weights, int dev
   if (mrn::gemm_prepare_device() != cudaSuccess || mrn::prepare_attention() != cudaSuccess)
     return bail(c->fail(MRN_ERR_CUDA, "kernel shared-memory attributes"));
   if (mrn::load_row_kernels(c->d) != cudaSuccess) return bail(c->fail(MRN_ERR_CUDA, "loading the row kernels failed"));
+  if (mrn::prepare_policy() != cudaSuccess) return bail(c->fail(MRN_ERR_CUDA, "loading the policy operators failed"));
   if (cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking) != cudaSuccess)
     return bail(c->fail(MRN_ERR_CUDA, "cudaStreamCreate failed"));
   if (cudaEventCreateWithFlags(&c->pass_done, cudaEventDisableTiming) != cudaSuccess)

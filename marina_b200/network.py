@@ -124,6 +124,22 @@ def c_arch(arch: Architecture):
     return ca, amax
 
 
+class LogitRules(_lib.MrnRules):
+    """What changes the logits of a batch of rows (`mrn_rules`): device pointers as integers, 0 or
+    None where a part is not used, with the lengths and strides that go with them. It holds no
+    reference to the memory; keep that alive while calls with the rules are in flight."""
+
+    def __init__(self, actions: int, **parts):
+        super().__init__(actions=actions)
+        for name, value in parts.items():
+            if name not in _RULE_PARTS:
+                raise TypeError(f"LogitRules has no part {name!r}: one of {sorted(_RULE_PARTS)}")
+            setattr(self, name, value)
+
+
+_RULE_PARTS = {name for name, _ in _lib.MrnRules._fields_} - {"actions"}
+
+
 class B200Network(Network):
     """One GPU's evaluator: `CudaNetwork::new(arch, &weights, ordinal, max_batch, fp8)`
     (src/net/cuda/mod.rs:276-493) with `precision` one of "bf16", "fp8w" (e4m3 weights,
@@ -225,6 +241,45 @@ class B200Network(Network):
         rc = self._lib.mrn_evaluate_device_static(self._ctx, n, c_void_p(boards_ptr), c_void_p(legal_ptr),
                                                   c_void_p(priors_ptr), c_void_p(wdl_ptr), c_void_p(stream or 0))
         self._check(rc, "static-scratch forward")
+
+    # -- policy operators (device pointers; enqueued on `stream`, the context's own if None) -----
+    def slot_table(self, rows: int, width: int, lengths_ptr: int, count: int, entries_ptr: int, starts_ptr: int,
+                   table_ptr: int, map_ptr: int | None = None, stream: int | None = None) -> None:
+        """`mrn_slot_table`: `rows` lists laid one behind the other in `entries` (int32, `count` in all)
+        into slot rows of `width`, -1 behind each list; `starts` [rows + 1] and the slot of each entry
+        in `map` [count], all int32."""
+        rc = self._lib.mrn_slot_table(self._ctx, rows, width, lengths_ptr, count, entries_ptr, starts_ptr, table_ptr,
+                                      map_ptr, stream)
+        self._check(rc, "slot table")
+
+    def adjust_logits(self, rows: int, width: int, logits_ptr: int, rules: LogitRules | None = None,
+                      out_ptr: int | None = None, priors_ptr: int | None = None, dtype: str = "f32",
+                      stride: int | None = None, out_stride: int | None = None, priors_stride: int | None = None,
+                      temperature_ptr: int | None = None, stream: int | None = None) -> None:
+        """`mrn_adjust_logits`: the logits (`dtype` "f32", "f16" or "bf16") under `rules` into `out` (the
+        same type; may be the logits themselves) and their softmax at each row's temperature into
+        `priors` (f32). Strides are in elements, `width` where not given."""
+        if dtype not in _lib.TYPES:
+            raise ValueError(f"dtype {dtype!r}: one of {sorted(_lib.TYPES)}")
+        rc = self._lib.mrn_adjust_logits(self._ctx, rows, width, logits_ptr, _lib.TYPES[dtype],
+                                         width if stride is None else stride, rules, temperature_ptr, out_ptr,
+                                         width if out_stride is None else out_stride, priors_ptr,
+                                         width if priors_stride is None else priors_stride, stream)
+        self._check(rc, "adjust logits")
+
+    def choose_actions(self, rows: int, width: int, logits_ptr: int, rules: LogitRules | None, column_ptr: int,
+                       action_ptr: int | None = None, prob_ptr: int | None = None, dtype: str = "f32",
+                       stride: int | None = None, temperature_ptr: int | None = None, top_k_ptr: int | None = None,
+                       top_p_ptr: int | None = None, uniform_ptr: int | None = None, stream: int | None = None) -> None:
+        """`mrn_choose_actions`: one column per row (int32, -1 where nothing is left), its action (int32)
+        and its share of the kept mass (f32), drawn with `uniform` [rows] from the logits under `rules`
+        at each row's temperature, within `top_k` (int32) and `top_p` (f32)."""
+        if dtype not in _lib.TYPES:
+            raise ValueError(f"dtype {dtype!r}: one of {sorted(_lib.TYPES)}")
+        rc = self._lib.mrn_choose_actions(self._ctx, rows, width, logits_ptr, _lib.TYPES[dtype],
+                                          width if stride is None else stride, rules, temperature_ptr, top_k_ptr,
+                                          top_p_ptr, uniform_ptr, column_ptr, action_ptr, prob_ptr, stream)
+        self._check(rc, "choose actions")
 
     def status_word(self) -> int:
         word = c_int()
