@@ -1,11 +1,15 @@
 // The policy operators; see policy.cuh for the arguments.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "kernels.cuh"
 #include "launch.h"
 #include "policy.cuh"
 #include "ptx.cuh"
+#include "rows.cuh"
 
 namespace mrn {
 
@@ -21,60 +25,141 @@ __device__ __forceinline__ int clamped_length(const SlotTableParams& p, int row)
   return n < 0 ? 0 : n > p.width ? p.width : n;
 }
 
-// starts[r] = lengths[0] + ... + lengths[r - 1]: one block walks the lengths 1024 at a time.
-__global__ void __launch_bounds__(1024) slot_starts_kernel(SlotTableParams p) {
-  __shared__ int warp_sum[32];
+// Exclusive sums of one value per thread in thread order, for a block of up to 32 warps;
+// *total gets the sum of all. `sums` is shared memory of 32.
+__device__ __forceinline__ int block_exclusive(int v, int* sums, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  int in = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(~0u, in, o);
+    if (lane >= o) in += u;
+  }
+  __syncthreads();
+  if (lane == 31) sums[warp] = in;
+  __syncthreads();
+  const int w = lane < warps ? sums[lane] : 0;
+  *total = __reduce_add_sync(~0u, w);
+  return __reduce_add_sync(~0u, lane < warp ? w : 0) + in - v;
+}
+
+__device__ __forceinline__ void flag_length(const SlotTableParams& p) {
+  if (p.status) atomicCAS(p.status, 0, kErrBadLength);
+}
+
+// One row of the table and the map, by one warp: table[r, s] = entries[first + s] for s < n, -1
+// behind; map[first + s] = r * width + s. QUADS: rows are 16-byte aligned, four slots to a store.
+template <bool QUADS>
+__device__ __forceinline__ void fill_row(const SlotTableParams& p, int row, int first, int n, int lane) {
+  const int at = row * p.width;  // rows * width < 2^31
+  const int listed = min(n, p.count - first);  // <= 0 where the entries ended before
+  if (QUADS) {
+    for (int s = 4 * lane; s < p.width; s += 128) {
+      int4 v = make_int4(-1, -1, -1, -1);
+      if (s < listed) v.x = __ldg(p.entries + first + s);
+      if (s + 1 < listed) v.y = __ldg(p.entries + first + s + 1);
+      if (s + 2 < listed) v.z = __ldg(p.entries + first + s + 2);
+      if (s + 3 < listed) v.w = __ldg(p.entries + first + s + 3);
+      *reinterpret_cast<int4*>(p.table + at + s) = v;
+    }
+  } else {
+    for (int s = lane; s < p.width; s += 32) p.table[at + s] = s < listed ? __ldg(p.entries + first + s) : -1;
+  }
+  if (p.map)
+    for (int s = lane; s < listed; s += 32) p.map[first + s] = at + s;
+}
+
+// Few rows: one launch. Block b lays out the rows [b * per, (b + 1) * per), per <= 32, and finds where
+// they start by adding up every length before them: reading up to 64 KB that all blocks share in L2
+// takes less time than a second launch.
+constexpr int kSlotsOneLaunch = 16384;
+
+template <bool QUADS>
+__global__ void __launch_bounds__(kThreads) slot_table_kernel(SlotTableParams p, int per) {
+  __shared__ int sums[32];
+  __shared__ int first[33];
   grid_dep_wait();
   grid_dep_launch();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int base = 0;
-  for (int r0 = 0; r0 < p.rows; r0 += 1024) {
-    const int row = r0 + tid;
-    int n = 0;
-    if (row < p.rows) {
-      n = clamped_length(p, row);
-      if (n != p.lengths[row] && p.status) atomicCAS(p.status, 0, kErrBadLength);
-    }
-    int v = n;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int r0 = blockIdx.x * per, r1 = min(r0 + per, p.rows);
+  int before = 0;
+  for (int r = tid; r < r0; r += kThreads) before += clamped_length(p, r);
+  int total;
+  block_exclusive(before, sums, &total);
+  if (tid < 32) {
+    const int row = r0 + lane;
+    const int n = row < r1 ? clamped_length(p, row) : 0;
+    if (row < r1 && n != p.lengths[row]) flag_length(p);
+    int in = n;
+#pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(~0u, v, o);
-      if (lane >= o) v += u;
+      const int u = __shfl_up_sync(~0u, in, o);
+      if (lane >= o) in += u;
     }
-    if (lane == 31) warp_sum[warp] = v;
-    __syncthreads();
-    if (warp == 0) {
-      int w = warp_sum[lane];
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(~0u, w, o);
-        if (lane >= o) w += u;
-      }
-      warp_sum[lane] = w;
+    first[lane] = total + in - n;
+    if (lane == 31) first[32] = total + in;
+    if (row < r1) p.starts[row] = total + in - n;
+    if (lane == 31 && r1 == p.rows) {
+      p.starts[p.rows] = total + in;
+      if (total + in > p.count) flag_length(p);
     }
-    __syncthreads();
-    const int before = base + (warp ? warp_sum[warp - 1] : 0) + v - n;
-    if (row < p.rows) p.starts[row] = before;
-    base += warp_sum[31];
-    __syncthreads();
   }
-  if (tid == 0) {
+  __syncthreads();
+  for (int row = r0 + (tid >> 5); row < r1; row += kWarps)
+    fill_row<QUADS>(p, row, first[row - r0], first[row - r0 + 1] - first[row - r0], lane);
+}
+
+// Many rows: the sums come first, by one cluster of eight blocks that each take an eighth of the rows,
+// add them up, exchange the eight sums through distributed shared memory and then write `starts`.
+constexpr int kScanBlocks = 8;
+
+__global__ void __cluster_dims__(kScanBlocks, 1, 1) __launch_bounds__(1024) slot_starts_kernel(SlotTableParams p) {
+  __shared__ int sums[32];
+  __shared__ int mine;
+  grid_dep_wait();
+  grid_dep_launch();
+  cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  const int tid = threadIdx.x, rank = cluster.block_rank();
+  const int64_t per = (static_cast<int64_t>(p.rows) + kScanBlocks - 1) / kScanBlocks;
+  const int64_t r0 = min(rank * per, static_cast<int64_t>(p.rows)), r1 = min(r0 + per, static_cast<int64_t>(p.rows));
+  int sum = 0, total;
+  for (int64_t r = r0 + tid; r < r1; r += 1024) sum += clamped_length(p, static_cast<int>(r));
+  block_exclusive(sum, sums, &total);
+  if (tid == 0) mine = total;
+  cluster.sync();
+  int base = 0;
+  for (int q = 0; q < rank; ++q) base += *cluster.map_shared_rank(&mine, q);
+  cluster.sync();  // no block leaves while another reads its sum
+  for (int64_t c = r0; c < r1; c += 1024) {
+    const int64_t row = c + tid;
+    int n = 0;
+    if (row < r1) {
+      n = clamped_length(p, static_cast<int>(row));
+      if (n != p.lengths[row]) flag_length(p);
+    }
+    const int at = base + block_exclusive(n, sums, &total);
+    if (row < r1) p.starts[row] = at;
+    base += total;
+  }
+  if (rank == kScanBlocks - 1 && tid == 0) {
     p.starts[p.rows] = base;
-    if (base > p.count && p.status) atomicCAS(p.status, 0, kErrBadLength);
+    if (base > p.count) flag_length(p);
   }
 }
 
-// table[r, s] = entries[starts[r] + s], -1 behind the list; map[starts[r] + s] = r * width + s.
-__global__ void __launch_bounds__(kThreads) slot_fill_kernel(SlotTableParams p) {
+// Then every warp lays out `per` <= 32 rows, whose starts it reads at once.
+template <bool QUADS>
+__global__ void __launch_bounds__(kThreads) slot_fill_kernel(SlotTableParams p, int per) {
   grid_dep_wait();
   grid_dep_launch();
   const int lane = threadIdx.x & 31;
-  const int row = blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (row >= p.rows) return;
-  const int first = p.starts[row], n = clamped_length(p, row);
-  const int64_t at = static_cast<int64_t>(row) * p.width;
-  for (int s = lane; s < p.width; s += 32) {
-    const bool listed = s < n && first + s < p.count;
-    p.table[at + s] = listed ? p.entries[first + s] : -1;
-    if (listed && p.map) p.map[first + s] = static_cast<int32_t>(at + s);
+  const int64_t r0 = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * per;
+  if (r0 >= p.rows) return;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(per), p.rows - r0));
+  const int here = lane < rows ? p.starts[r0 + lane] : 0, next = lane < rows ? p.starts[r0 + lane + 1] : 0;
+  for (int i = 0; i < rows; ++i) {
+    const int first = __shfl_sync(~0u, here, i);
+    fill_row<QUADS>(p, static_cast<int>(r0) + i, first, __shfl_sync(~0u, next, i) - first, lane);
   }
 }
 
@@ -207,6 +292,397 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
+// ---- the choice of an action -----------------------------------------------------------
+// Weights are whole numbers, 2^40 for the largest logit: their sums are exact in any order, so the
+// column that a uniform number falls on does not depend on how the row was split. The exponential
+// is computed in f64: an error of 2^-24 in it would move the borders between columns by as much,
+// and a row in a million would fall on another column than by the definition.
+constexpr double kWeightOne = 1099511627776.0;  // 2^40; a row's 2^18 columns sum to at most 2^58
+
+struct Weights {
+  double m, inv_t;
+  bool infinite;  // the largest logit is +inf: the columns that hold it share the row
+  __device__ __forceinline__ uint64_t operator()(float x) const {
+    if (!(x > -INFINITY)) return 0;
+    if (infinite) return x == INFINITY ? static_cast<uint64_t>(kWeightOne) : 0;
+    return static_cast<uint64_t>(__double2ll_rn(exp((static_cast<double>(x) - m) * inv_t) * kWeightOne));
+  }
+};
+
+// ---- narrow rows: one warp each ------------------------------------------------------------
+// A row of up to 512 columns (a slot row has 224) stays in the registers of one warp, column
+// 32 k + lane in v[k]: nothing but warp shuffles between its steps, and every global read of the row
+// in flight at once. COLUMNS = K * 32 is the widest row of an instantiation.
+constexpr int kNarrowWarps = 4;
+
+// A warp's shared memory: a hash table from action to count (for slots; linear probing, at most half
+// full, so that a probe always ends), or a count for each column; then, for the choice, the columns
+// that are left.
+template <int K>
+struct NarrowShared {
+  static constexpr int kEntries = 64 * K;  // twice the columns, a power of two
+  union {
+    struct {
+      int keys[kEntries];
+      int counts[kEntries];
+    };
+    struct {
+      uint64_t kept[32 * K];  // weight of the i-th column that is left, 0 once it is cut off
+      float x[32 * K];
+      int column[32 * K];
+    };
+  };
+
+  static __device__ __forceinline__ unsigned slot(int action) {
+    return (static_cast<unsigned>(action) * 2654435761u) >> 16 & (kEntries - 1);  // Knuth's multiplicative hash
+  }
+  __device__ __forceinline__ int insert(int action) {
+    unsigned h = slot(action);
+    for (;;) {
+      const int was = atomicCAS(&keys[h], -1, action);
+      if (was == -1 || was == action) return h;
+      h = (h + 1) & (kEntries - 1);
+    }
+  }
+  __device__ __forceinline__ int find(int action) const {
+    unsigned h = slot(action);
+    for (;;) {
+      const int k = keys[h];
+      if (k == action) return h;
+      if (k == -1) return -1;
+      h = (h + 1) & (kEntries - 1);
+    }
+  }
+};
+
+// Adjusted logits of a row.
+template <class T, int K, bool SLOTS>
+__device__ __forceinline__ void load_narrow(const LogitParams& p, int row, int lane, NarrowShared<K>& sh, float (&v)[K]) {
+  const RuleParams& r = p.rules;
+  const T* logits = static_cast<const T*>(p.logits) + row * p.stride;
+  const Penalties pen = row_penalties(r, row);
+  const uint32_t* mask = r.mask ? r.mask + row * r.mask_stride : nullptr;
+  int a[K], at[K];  // the column's action, -1 where it is masked or empty; its count's place
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = 32 * k + lane;
+    a[k] = -1;
+    v[k] = 0.f;
+    if (c < p.width) {
+      a[k] = SLOTS ? r.columns[row * r.columns_stride + c] : c;
+      v[k] = as_float(logits[c]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if (SLOTS && a[k] >= r.actions) {
+      if (p.status) atomicCAS(p.status, 0, kErrBadAction);
+      a[k] = -1;
+    }
+    at[k] = 32 * k + lane;
+    if (mask && a[k] >= 0 && !((mask[a[k] >> 5] >> (a[k] & 31)) & 1)) a[k] = -1;
+  }
+  const int biases = r.bias_len;
+  if (pen.seen > 0 || (SLOTS && biases)) {
+    if (SLOTS) {
+#pragma unroll
+      for (int i = 0; i < 2 * K; ++i) sh.keys[32 * i + lane] = -1, sh.counts[32 * i + lane] = 0;
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k) sh.counts[32 * k + lane] = 0;
+    }
+    __syncwarp();
+    if (SLOTS) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (a[k] >= 0) at[k] = sh.insert(a[k]);
+      __syncwarp();
+    }
+    const int32_t* history = r.history + row * r.history_stride;
+    for (int e = lane; e < pen.seen; e += 32) {
+      const int id = history[e];
+      const int h = id < 0 ? -1 : SLOTS ? sh.find(id) : id < p.width ? id : -1;
+      if (h >= 0) atomicAdd(&sh.counts[h], 1);
+    }
+    __syncwarp();
+    if (pen.seen > 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (a[k] >= 0) v[k] = penalised(v[k], sh.counts[at[k]], pen);
+    }
+  }
+  // Biases in the list's order: every lane looks one entry up, and the ones that name a column are
+  // added one after the other.
+  for (int e0 = 0; e0 < biases; e0 += 32) {
+    const int e = e0 + lane;
+    const int id = e < biases ? r.bias_actions[row * r.bias_stride + e] : -1;
+    const float value = e < biases ? r.bias_values[row * r.bias_stride + e] : 0.f;
+    const int h = id < 0 ? -1 : SLOTS ? sh.find(id) : id < p.width ? id : -1;
+    unsigned todo = __ballot_sync(~0u, h >= 0);
+    while (todo) {
+      const int j = __ffs(todo) - 1;
+      todo &= todo - 1;
+      const int place = __shfl_sync(~0u, h, j);
+      const float add = __shfl_sync(~0u, value, j);
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (at[k] == place && a[k] >= 0) v[k] = __fadd_rn(v[k], add);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    if (a[k] < 0) v[k] = -INFINITY;
+}
+
+template <class T, int K, bool SLOTS>
+__global__ void __launch_bounds__(kNarrowWarps * 32) adjust_narrow_kernel(AdjustParams p) {
+  __shared__ NarrowShared<K> shared[kNarrowWarps];
+  grid_dep_wait();
+  grid_dep_launch();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = blockIdx.x * kNarrowWarps + warp;
+  if (row >= p.in.rows) return;
+  const int width = p.in.width;
+  float v[K];
+  load_narrow<T, K, SLOTS>(p.in, row, lane, shared[warp], v);
+  if (p.out) {
+    T* out = static_cast<T*>(p.out) + row * p.out_stride;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (32 * k + lane < width) from_float(v[k], out + 32 * k + lane);
+  }
+  if (!p.priors) return;
+  const float t = p.in.temperature ? p.in.temperature[row] : 1.f;
+  float m = -INFINITY;
+  bool nan = t != t;
+#pragma unroll
+  for (int k = 0; k < K; ++k) m = fmaxf(m, v[k]), nan |= v[k] != v[k];
+  m = warp_max(m);
+  nan = __any_sync(~0u, nan);
+  float* priors = p.priors + row * p.priors_stride;
+  float e[K];
+  if (t <= 0.f && !nan) {  // the lowest column of the largest logit
+    int first = kPolicyMaxWidth;
+#pragma unroll
+    for (int k = K - 1; k >= 0; --k)
+      if (v[k] == m && m > -INFINITY) first = 32 * k + lane;
+    first = __reduce_min_sync(~0u, first);
+#pragma unroll
+    for (int k = 0; k < K; ++k) e[k] = 32 * k + lane == first ? 1.f : 0.f;
+  } else {
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      e[k] = v[k] == -INFINITY ? 0.f : v[k] == m ? 1.f : m == INFINITY ? 0.f : expf((v[k] - m) / t);
+      sum += e[k];
+    }
+    sum = warp_sum(sum);
+    const float inv = nan ? NAN : sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int k = 0; k < K; ++k) e[k] = v[k] == -INFINITY ? 0.f : e[k] * inv;
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    if (32 * k + lane < width) priors[32 * k + lane] = e[k];
+}
+
+struct Choice {
+  int column;  // -1: nothing is left, or a NaN
+  float prob;
+};
+
+__device__ __forceinline__ void write_choice(const ChooseParams& p, int row, Choice c) {
+  p.column[row] = c.column;
+  if (p.action) {
+    const RuleParams& r = p.in.rules;
+    p.action[row] = c.column < 0 || !r.columns ? c.column : r.columns[row * r.columns_stride + c.column];
+  }
+  if (p.prob) p.prob[row] = c.prob;
+}
+
+__device__ __forceinline__ uint64_t warp_sum_u64(uint64_t v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  return v;
+}
+
+// Exclusive sums over the lanes.
+__device__ __forceinline__ uint64_t warp_exclusive_u64(uint64_t v, int lane) {
+  uint64_t in = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint64_t u = __shfl_up_sync(~0u, in, o);
+    if (lane >= o) in += u;
+  }
+  return in - v;
+}
+
+// The whole number of weight units that a share of the mass needs.
+__device__ __forceinline__ uint64_t needed_mass(float top_p, uint64_t mass) {
+  const double want = ceil(static_cast<double>(top_p) * static_cast<double>(mass));
+  return want < 1.0 ? 1 : min(static_cast<uint64_t>(want), mass);
+}
+
+__device__ __forceinline__ uint64_t drawn_unit(float uniform, uint64_t mass) {
+  const double at = static_cast<double>(uniform) * static_cast<double>(mass);
+  return at > 0.0 ? min(static_cast<uint64_t>(at), mass - 1) : 0;
+}
+
+// Draws from the `left` <= 32 G columns in sh.x, which are in column order. With a cut-off they are
+// sorted by (logit, lower column) in a bitonic network, 32 G elements in the order i = lane G + g:
+// exchanges at a distance below G stay in a thread, the others are shuffles. A weight is computed
+// once for each column.
+template <int G, int K>
+__device__ __forceinline__ Choice draw_narrow(const ChooseParams& p, int row, int lane, NarrowShared<K>& sh, int left,
+                                              const Weights& weight) {
+  const int k = p.top_k ? p.top_k[row] : 0;
+  const float top_p = p.top_p ? p.top_p[row] : 1.f;
+  uint64_t kept[G];
+  uint64_t total;
+  if ((k > 0 && k < left) || top_p < 1.f) {
+    uint64_t e[G];  // order key, then the complement of the place: larger is earlier
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const int i = lane * G + g;
+      e[g] = i < left ? static_cast<uint64_t>(order_key(sh.x[i])) << 32 | ~static_cast<uint32_t>(i) : 0;
+    }
+#pragma unroll
+    for (int size = 2; size <= 32 * G; size <<= 1) {
+#pragma unroll
+      for (int d = size >> 1; d; d >>= 1) {
+        if (d >= G) {
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            const uint64_t o = __shfl_xor_sync(~0u, e[g], d / G);
+            const int i = lane * G + g;
+            const bool larger = ((i & d) == 0) == ((i & size) == 0 || size == 32 * G);
+            e[g] = (e[g] > o) == larger ? e[g] : o;
+          }
+        } else {
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+            if (!(g & d)) {
+              const int i = lane * G + g;
+              const bool down = (i & size) == 0 || size == 32 * G;
+              const uint64_t x = e[g], y = e[g | d];
+              const bool swap = (x < y) == down;
+              e[g] = swap ? y : x;
+              e[g | d] = swap ? x : y;
+            }
+        }
+      }
+    }
+    const int most = k > 0 ? min(k, left) : left;
+    uint64_t mine = 0;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      kept[g] = lane * G + g < most ? weight(key_value(static_cast<uint32_t>(e[g] >> 32))) : 0;
+      mine += kept[g];
+    }
+    uint64_t ahead = warp_exclusive_u64(mine, lane);
+    total = __shfl_sync(~0u, ahead + mine, 31);
+    if (top_p < 1.f) {
+      const uint64_t need = needed_mass(top_p, total);
+      mine = 0;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const uint64_t w = kept[g];
+        if (ahead >= need) kept[g] = 0;
+        ahead += w;
+        mine += kept[g];
+      }
+      total = warp_sum_u64(mine);
+    }
+    // back to column order
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+      if (lane * G + g < left) sh.kept[~static_cast<uint32_t>(e[g])] = kept[g];
+    __syncwarp();
+#pragma unroll
+    for (int g = 0; g < G; ++g) kept[g] = lane * G + g < left ? sh.kept[lane * G + g] : 0;
+  } else {
+    uint64_t mine = 0;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      kept[g] = lane * G + g < left ? weight(sh.x[lane * G + g]) : 0;
+      mine += kept[g];
+    }
+    total = warp_sum_u64(mine);
+  }
+  if (!p.uniform) return Choice{-1, static_cast<float>(kWeightOne / static_cast<double>(total))};  // the largest's
+  const uint64_t unit = drawn_unit(p.uniform[row], total);
+  uint64_t mine = 0;
+#pragma unroll
+  for (int g = 0; g < G; ++g) mine += kept[g];
+  uint64_t ahead = warp_exclusive_u64(mine, lane);
+  int place = -1;
+  uint64_t w = 0;
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    if (place < 0 && unit >= ahead && unit < ahead + kept[g]) place = lane * G + g, w = kept[g];
+    ahead += kept[g];
+  }
+  const int owner = __ffs(__ballot_sync(~0u, place >= 0)) - 1;
+  place = __shfl_sync(~0u, place, owner);
+  w = __shfl_sync(~0u, w, owner);
+  return Choice{sh.column[place], static_cast<float>(static_cast<double>(w) / static_cast<double>(total))};
+}
+
+template <class T, int K, bool SLOTS>
+__global__ void __launch_bounds__(kNarrowWarps * 32) choose_narrow_kernel(ChooseParams p) {
+  __shared__ NarrowShared<K> shared[kNarrowWarps];
+  grid_dep_wait();
+  grid_dep_launch();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = blockIdx.x * kNarrowWarps + warp;
+  if (row >= p.in.rows) return;
+  NarrowShared<K>& sh = shared[warp];
+  float v[K];
+  load_narrow<T, K, SLOTS>(p.in, row, lane, sh, v);
+  __syncwarp();
+  const float t = p.in.temperature ? p.in.temperature[row] : 1.f;
+  float m = -INFINITY;
+  bool nan = t != t;
+  int left = 0;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    m = fmaxf(m, v[k]), nan |= v[k] != v[k];
+    const unsigned here = __ballot_sync(~0u, v[k] > -INFINITY);
+    if (v[k] > -INFINITY) {
+      const int i = left + __popc(here & ((1u << lane) - 1));
+      sh.x[i] = v[k], sh.column[i] = 32 * k + lane;
+    }
+    left += __popc(here);
+  }
+  m = warp_max(m);
+  nan = __any_sync(~0u, nan);
+  __syncwarp();
+  Choice c{-1, nan ? NAN : 0.f};
+  if (!nan && left) {
+    if (t <= 0.f || !p.uniform) {
+      int first = kPolicyMaxWidth;
+#pragma unroll
+      for (int k = K - 1; k >= 0; --k)
+        if (v[k] == m) first = 32 * k + lane;
+      c.column = __reduce_min_sync(~0u, first);
+      c.prob = 1.f;
+    }
+    if (t > 0.f) {
+      const Weights weight{static_cast<double>(m), 1.0 / static_cast<double>(t), m == INFINITY};
+      Choice d;
+      if (K == 1 || left <= 32) d = draw_narrow<1, K>(p, row, lane, sh, left, weight);
+      else if (K == 2 || left <= 64) d = draw_narrow<2, K>(p, row, lane, sh, left, weight);
+      else if (K == 4 || left <= 128) d = draw_narrow<4, K>(p, row, lane, sh, left, weight);
+      else if (K == 8 || left <= 256) d = draw_narrow<8, K>(p, row, lane, sh, left, weight);
+      else d = draw_narrow<16, K>(p, row, lane, sh, left, weight);
+      if (!p.uniform) d.column = c.column;
+      c = d;
+    }
+  }
+  if (lane == 0) write_choice(p, row, c);
+}
+
+// ---- wide rows -------------------------------------------------------------------------
 template <class T>
 __global__ void __launch_bounds__(kThreads) adjust_kernel(AdjustParams p) {
   __shared__ float x[kChunk];
@@ -219,7 +695,7 @@ __global__ void __launch_bounds__(kThreads) adjust_kernel(AdjustParams p) {
   float m = 0.f, inv = 0.f;
   int first = -1;
   // exp((v - m) / t); a largest logit of +inf is shared by the columns that hold it
-  auto relative = [&](float v) { return v == m ? 1.f : m == INFINITY ? v * 0.f : expf((v - m) / t); };
+  auto relative = [&](float v) { return v == m ? 1.f : m == INFINITY ? 0.f : expf((v - m) / t); };
   if (p.priors) {
     bool nan;
     const uint64_t best = row_maximum<T>(p.in, pen, row, x, shared, &nan);
@@ -256,23 +732,6 @@ __global__ void __launch_bounds__(kThreads) adjust_kernel(AdjustParams p) {
     }
   }
 }
-
-// ---- the choice of an action -----------------------------------------------------------
-// Weights are whole numbers, 2^40 for the largest logit: their sums are exact in any order, so the
-// column that a uniform number falls on does not depend on how the row was split. The exponential
-// is computed in f64: an error of 2^-24 in it would move the borders between columns by as much,
-// and a row in a million would fall on another column than by the definition.
-constexpr double kWeightOne = 1099511627776.0;  // 2^40; a row's 2^18 columns sum to at most 2^58
-
-struct Weights {
-  double m, inv_t;
-  bool infinite;  // the largest logit is +inf: the columns that hold it share the row
-  __device__ __forceinline__ uint64_t operator()(float x) const {
-    if (!(x > -INFINITY)) return 0;
-    if (infinite) return x == INFINITY ? static_cast<uint64_t>(kWeightOne) : 0;
-    return static_cast<uint64_t>(__double2ll_rn(exp((static_cast<double>(x) - m) * inv_t) * kWeightOne));
-  }
-};
 
 template <class T>
 __global__ void __launch_bounds__(kThreads) choose_kernel(ChooseParams p) {
@@ -451,21 +910,63 @@ cudaError_t with_type(LogitType t, F&& f) {
   return cudaErrorInvalidValue;
 }
 
+template <int N>
+using Int = std::integral_constant<int, N>;
+
+// Widest row of the one-warp kernels.
+constexpr int kNarrowWidth = 512;
+
+dim3 narrow_grid(int rows) { return dim3((rows + kNarrowWarps - 1) / kNarrowWarps); }
+
+// f(type, columns / 32, whether columns are slots) for the narrow kernels' instantiations.
+template <class F>
+cudaError_t with_narrow(const LogitParams& p, F&& f) {
+  return with_type(p.type, [&](auto v) {
+    auto with_width = [&](auto slots) {
+      if (p.width <= 64) return f(v, Int<2>(), slots);
+      if (p.width <= 256) return f(v, Int<8>(), slots);
+      return f(v, Int<16>(), slots);
+    };
+    return p.rules.columns ? with_width(std::true_type()) : with_width(std::false_type());
+  });
+}
+
 }  // namespace
 
 cudaError_t launch_slot_table(const SlotTableParams& p, cudaStream_t s) {
-  cudaError_t e = launch_kernel(slot_starts_kernel, dim3(1), dim3(1024), 0, s, p);
-  if (e != cudaSuccess || p.rows == 0) return e;
-  return launch_kernel(slot_fill_kernel, dim3((p.rows + kWarps - 1) / kWarps), dim3(kThreads), 0, s, p);
+  const bool quads = p.width % 4 == 0 && reinterpret_cast<uintptr_t>(p.table) % 16 == 0;
+  if (p.rows <= kSlotsOneLaunch) {
+    const int per = p.rows <= 2048 ? 4 : p.rows <= 8192 ? 8 : 32;
+    const int blocks = p.rows ? (p.rows + per - 1) / per : 1;
+    return launch_kernel(quads ? slot_table_kernel<true> : slot_table_kernel<false>, dim3(blocks), dim3(kThreads), 0, s, p,
+                         per);
+  }
+  const cudaError_t e = launch_kernel(slot_starts_kernel, dim3(kScanBlocks), dim3(1024), 0, s, p);
+  if (e != cudaSuccess) return e;
+  const PdlScope pdl(true);  // the second kernel waits for the first before it reads `starts`
+  const int per = 8;
+  const int64_t warps = (static_cast<int64_t>(p.rows) + per - 1) / per;
+  return launch_kernel(quads ? slot_fill_kernel<true> : slot_fill_kernel<false>,
+                       dim3(static_cast<unsigned>((warps + kWarps - 1) / kWarps)), dim3(kThreads), 0, s, p, per);
 }
 
 cudaError_t launch_adjust(const AdjustParams& p, cudaStream_t s) {
+  if (p.in.width <= kNarrowWidth)
+    return with_narrow(p.in, [&](auto v, auto k, auto slots) {
+      return launch_kernel(adjust_narrow_kernel<decltype(v), k.value, slots.value>, narrow_grid(p.in.rows),
+                           dim3(kNarrowWarps * 32), 0, s, p);
+    });
   return with_type(p.in.type, [&](auto v) {
     return launch_kernel(adjust_kernel<decltype(v)>, dim3(p.in.rows), dim3(kThreads), 0, s, p);
   });
 }
 
 cudaError_t launch_choose(const ChooseParams& p, cudaStream_t s) {
+  if (p.in.width <= kNarrowWidth)
+    return with_narrow(p.in, [&](auto v, auto k, auto slots) {
+      return launch_kernel(choose_narrow_kernel<decltype(v), k.value, slots.value>, narrow_grid(p.in.rows),
+                           dim3(kNarrowWarps * 32), 0, s, p);
+    });
   return with_type(p.in.type, [&](auto v) {
     return launch_kernel(choose_kernel<decltype(v)>, dim3(p.in.rows), dim3(kThreads), 0, s, p);
   });
@@ -475,8 +976,22 @@ cudaError_t prepare_policy() {
   cudaFuncAttributes a;
   cudaError_t e;
   if ((e = cudaFuncGetAttributes(&a, slot_starts_kernel)) != cudaSuccess) return e;
-  if ((e = cudaFuncGetAttributes(&a, slot_fill_kernel)) != cudaSuccess) return e;
+  if ((e = cudaFuncGetAttributes(&a, slot_fill_kernel<true>)) != cudaSuccess) return e;
+  if ((e = cudaFuncGetAttributes(&a, slot_fill_kernel<false>)) != cudaSuccess) return e;
+  if ((e = cudaFuncGetAttributes(&a, slot_table_kernel<true>)) != cudaSuccess) return e;
+  if ((e = cudaFuncGetAttributes(&a, slot_table_kernel<false>)) != cudaSuccess) return e;
   for (LogitType t : {LogitType::kF32, LogitType::kF16, LogitType::kBf16}) {
+    for (int width : {64, 256, 512})
+      for (bool slots : {false, true}) {
+        LogitParams in{};
+        const int32_t some = 0;
+        in.type = t, in.width = width, in.rules.columns = slots ? &some : nullptr;
+        e = with_narrow(in, [&](auto v, auto k, auto sl) {
+          const cudaError_t r = cudaFuncGetAttributes(&a, adjust_narrow_kernel<decltype(v), k.value, sl.value>);
+          return r != cudaSuccess ? r : cudaFuncGetAttributes(&a, choose_narrow_kernel<decltype(v), k.value, sl.value>);
+        });
+        if (e != cudaSuccess) return e;
+      }
     e = with_type(t, [&](auto v) {
       const cudaError_t r = cudaFuncGetAttributes(&a, adjust_kernel<decltype(v)>);
       return r != cudaSuccess ? r : cudaFuncGetAttributes(&a, choose_kernel<decltype(v)>);
