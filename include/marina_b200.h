@@ -274,8 +274,9 @@ typedef enum mrn_type {
   MRN_TYPE_BF16 = 2,
 } mrn_type;
 
-/* Columns a row of the policy operators may have. */
+/* Columns a row of mrn_adjust_logits and mrn_choose_actions may have, and rows of a call. */
 #define MRN_MAX_WIDTH (1 << 18)
+#define MRN_MAX_ROWS (1 << 27)
 
 /* What changes the logits of a batch of rows. Strides count elements between rows; a stride of 0
  * makes every row share one list. Unused parts are NULL (or have length 0).

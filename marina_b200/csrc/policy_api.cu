@@ -9,7 +9,7 @@
 
 namespace mrn {
 
-static_assert(MRN_MAX_WIDTH == kPolicyMaxWidth, "the header's widest row is the kernels'");
+static_assert(MRN_MAX_WIDTH == kPolicyMaxWidth && MRN_MAX_ROWS == kPolicyMaxRows, "the header's limits are the kernels'");
 
 namespace {
 
@@ -83,7 +83,7 @@ namespace {
 
 int logit_params(mrn_ctx* c, int rows, int width, const void* logits, int type, int64_t stride, const mrn_rules* rules,
                  const float* temperature, LogitParams* out) {
-  if (rows < 0) return c->fail(MRN_ERR_ARGUMENT, "rows = %d", rows);
+  if (rows < 0 || rows > kPolicyMaxRows) return c->fail(MRN_ERR_ARGUMENT, "rows = %d (0..%d)", rows, kPolicyMaxRows);
   if (width < 1 || width > MRN_MAX_WIDTH) return c->fail(MRN_ERR_ARGUMENT, "width %d (1..%d)", width, MRN_MAX_WIDTH);
   if (type < MRN_TYPE_F32 || type > MRN_TYPE_BF16) return c->fail(MRN_ERR_ARGUMENT, "unknown type %d", type);
   if (stride < 0 || (stride > 0 && stride < width))
@@ -92,7 +92,7 @@ int logit_params(mrn_ctx* c, int rows, int width, const void* logits, int type, 
   if (misaligned(logits, type == MRN_TYPE_F32 ? 4 : 2) || misaligned(temperature, 4))
     return c->fail(MRN_ERR_ARGUMENT, "logits or temperature is not aligned to its elements");
   out->logits = logits, out->type = static_cast<LogitType>(type), out->stride = stride;
-  out->rows = rows, out->width = width, out->temperature = temperature, out->status = c->status;
+  out->rows = rows, out->width = width, out->temperature = temperature, out->status = c->status, out->sms = c->num_sms;
   return rule_params(c, rows, width, rules, &out->rules);
 }
 

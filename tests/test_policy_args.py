@@ -98,7 +98,8 @@ def test_rules_that_are_fine(net):
 
 
 @pytest.mark.parametrize("change,words", [
-    ({"rows": -1}, "rows = -1"), ({"width": 0}, "width 0"), ({"width": (1 << 18) + 1, "stride": 1 << 20}, "width 262145"),
+    ({"rows": -1}, "rows = -1"), ({"rows": (1 << 27) + 1, "stride": 0}, "rows = 134217729"), ({"width": 0}, "width 0"),
+    ({"width": (1 << 18) + 1, "stride": 1 << 20}, "width 262145"),
     ({"logits_ptr": None}, "logits is NULL"), ({"stride": 223}, "stride 223"), ({"stride": -224}, "stride -224"),
     ({"logits_ptr": P + 1}, "aligned"), ({"temperature_ptr": P + 2}, "aligned"),
 ])
