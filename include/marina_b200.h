@@ -350,6 +350,26 @@ MRN_API int mrn_choose_actions(mrn_ctx* ctx, int rows, int width, const void* lo
                                const float* top_p, const float* uniform, int32_t* column, int32_t* action, float* prob,
                                void* stream);
 
+/* `mrn_evaluate` on move lists as a search holds them, from host memory: lengths[p] legal actions of
+ * position p (0 .. MRN_MAX_LEGAL), the lists of all positions one behind the other in `actions`. The
+ * slot rows are built on the GPU, so that a call moves about 30 actions and priors a position across
+ * the bus instead of 224 of each. `rules` (NULL: none) and `temperature` (NULL: 1) are as for
+ * mrn_adjust_logits, with every pointer to host memory, `actions` MRN_ACTIONS and `columns` NULL: the
+ * moves are the columns. `priors` gets one prior per listed action, in the lists' order; `wdl` is n x 3.
+ * Without rules and temperature the priors are mrn_evaluate's up to f32 rounding. Synchronous; the
+ * first call allocates a max_batch x 224 x 4-byte device buffer and records the pass of its batch
+ * size again, and calls with more moves or longer lists than any before allocate for them. */
+MRN_API int mrn_evaluate_moves(mrn_ctx* ctx, int n, const uint8_t* boards, const int32_t* lengths, const int32_t* actions,
+                               const mrn_rules* rules, const float* temperature, float* priors, float* wdl);
+
+/* One move per position, as mrn_choose_actions draws it from the position's list: move[p] is its place
+ * in the list, -1 where the list is empty or the rules leave nothing of it; prob[p] (NULL: not wanted)
+ * its share of the kept mass. Arguments as for mrn_evaluate_moves; top_k, top_p and uniform [n], in
+ * host memory, or NULL. */
+MRN_API int mrn_choose_moves(mrn_ctx* ctx, int n, const uint8_t* boards, const int32_t* lengths, const int32_t* actions,
+                             const mrn_rules* rules, const float* temperature, const int32_t* top_k, const float* top_p,
+                             const float* uniform, int32_t* move, float* prob, float* wdl);
+
 #ifdef __cplusplus
 }
 #endif

@@ -41,7 +41,7 @@ EXPORTS = (
     "mrn_group_create", "mrn_group_evaluate", "mrn_group_size", "mrn_group_context", "mrn_group_describe",
     "mrn_group_last_error", "mrn_group_destroy",
     "mrn_evaluate_device_static",
-    "mrn_slot_table", "mrn_adjust_logits", "mrn_choose_actions",
+    "mrn_slot_table", "mrn_adjust_logits", "mrn_choose_actions", "mrn_evaluate_moves", "mrn_choose_moves",
 )
 TEST_EXPORTS = ("mrn_test_gemm", "mrn_test_gemm_wait_expiry", "mrn_test_attention", "mrn_test_layernorm",
                 "mrn_test_context", "mrn_test_context_error", "mrn_test_context_free", "mrn_test_last_error")
@@ -104,6 +104,10 @@ SIGNATURES = {
                                   c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
     "mrn_choose_actions": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int, c_int64, POINTER(MrnRules), c_void_p,
                                    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "mrn_evaluate_moves": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, POINTER(MrnRules), c_void_p, c_void_p,
+                                   c_void_p]),
+    "mrn_choose_moves": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, POINTER(MrnRules), c_void_p, c_void_p,
+                                 c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "mrn_group_create": (c_int, [POINTER(MrnArch), POINTER(MrnWeights), POINTER(c_int), c_int, c_int, c_int,
                                  POINTER(c_void_p)]),
     "mrn_group_evaluate": (c_int, [c_void_p, c_int, POINTER(c_uint8), POINTER(c_int32), POINTER(c_float),

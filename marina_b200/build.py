@@ -32,7 +32,7 @@ TEST_LIB = PKG / "libmarina_b200_test.so"
 CHESS_LIB = PKG / "libmarina_chess.so"
 
 CUDA_SOURCES = ["gemm.cu", "kernels.cu", "attention.cu", "runtime.cu", "static_forward.cu", "group.cpp",
-                "policy.cu", "policy_wide.cu", "policy_api.cu"]
+                "policy.cu", "policy_wide.cu", "policy_api.cu", "moves.cu"]
 TEST_SOURCES = ["gemm.cu", "kernels.cu", "attention.cu", "policy.cu", "policy_wide.cu", "policy_api.cu", "api_test.cu"]
 CUDA_HEADERS = ["ptx.cuh", "rows.cuh", "e4m3x2.cuh", "gemm.cuh", "gemm.h", "tmap.h", "kernels.cuh", "launch.h", "runtime.h",
                 "policy.cuh", "policy_rows.cuh", "policy_api.h"]

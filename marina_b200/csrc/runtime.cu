@@ -353,9 +353,13 @@ int make_plans(mrn_ctx* c, Bucket& b) {
   return MRN_OK;
 }
 
-// The whole forward pass of one bucket on `s`. `logits_out`, when set, selects raw logits over
-// all actions ([positions, 4672]) and raw WDL logits instead of priors and probabilities.
-int enqueue(mrn_ctx* c, Bucket& b, cudaStream_t s, float* logits_out, Profiler* prof) {
+// What the heads of a pass write: priors of the legal slots and WDL probabilities; raw logits of
+// all actions ([positions, 4672]) and raw WDL logits; or raw logits of the legal slots and WDL
+// probabilities.
+enum class HeadsOut { kPriors, kAllLogits, kSlotLogits };
+
+// The whole forward pass of one bucket on `s`, the policy into `policy`.
+int enqueue(mrn_ctx* c, Bucket& b, cudaStream_t s, HeadsOut heads, float* policy, Profiler* prof) {
   const int P = b.positions, R = P * c->t, d = c->d;
   const ActType act = c->act;
   auto mark = [&](int cls) {
@@ -403,15 +407,16 @@ int enqueue(mrn_ctx* c, Bucket& b, cudaStream_t s, float* logits_out, Profiler* 
   mrn::HeadsParams hp;
   hp.x = c->x, hp.final_g = c->fn_g, hp.final_b = c->fn_b, hp.policy_g = c->pn_g, hp.policy_b = c->pn_b;
   hp.policy_w = c->pw, hp.policy_bias = c->pb, hp.value_g = c->vn_g, hp.value_b = c->vn_b;
-  hp.legal = logits_out ? nullptr : c->legal;
-  hp.slots = logits_out ? MRN_ACTIONS : MRN_MAX_LEGAL;
-  hp.softmax = logits_out ? 0 : 1;
-  hp.priors = logits_out ? logits_out : c->priors;
+  const bool all = heads == HeadsOut::kAllLogits;
+  hp.legal = all ? nullptr : c->legal;
+  hp.slots = all ? MRN_ACTIONS : MRN_MAX_LEGAL;
+  hp.softmax = heads == HeadsOut::kPriors ? 1 : 0;
+  hp.priors = policy;
   hp.value_in = c->vnorm, hp.status = c->status, hp.eps = c->eps, hp.t = c->t, hp.square_start = c->square_start;
   mark(MRN_PROFILE_HEADS);
   CK(mrn::launch_heads(hp, P, d, s));
   CK(mrn::gemm_launch(b.plans[4 * c->layers], s));
-  CK(mrn::launch_value_out(mrn::ValueOutParams{c->vhid, c->vw2, c->vb2, c->wdl, logits_out ? 0 : 1}, P, d, s));
+  CK(mrn::launch_value_out(mrn::ValueOutParams{c->vhid, c->vw2, c->vb2, c->wdl, all ? 0 : 1}, P, d, s));
   done();
   return MRN_OK;
 }
@@ -419,6 +424,23 @@ int enqueue(mrn_ctx* c, Bucket& b, cudaStream_t s, float* logits_out, Profiler* 
 // Embedding; per layer QKV, attention, out-proj, norm2, FFN1, FFN2; norm1 of every layer but the
 // first; 3 for the heads.
 int launches_per_forward(const mrn_ctx* c) { return 1 + 6 * c->layers + (c->layers - 1) + 3; }
+
+// Captures the pass of bucket `b` into a graph (src/net/cuda/mod.rs:689-700).
+int capture(mrn_ctx* c, Bucket& b, HeadsOut heads, float* policy, cudaGraphExec_t* out) {
+  CK(cudaStreamBeginCapture(c->stream, cudaStreamCaptureModeThreadLocal));
+  const int rc = enqueue(c, b, c->stream, heads, policy, nullptr);
+  cudaGraph_t graph = nullptr;
+  const cudaError_t end = cudaStreamEndCapture(c->stream, &graph);
+  if (rc) {
+    if (graph) cudaGraphDestroy(graph);
+    return rc;
+  }
+  if (end != cudaSuccess || !graph) return c->fail(MRN_ERR_CUDA, "graph capture failed: %s", cudaGetErrorString(end));
+  const cudaError_t inst = cudaGraphInstantiate(out, graph, 0);
+  cudaGraphDestroy(graph);
+  if (inst != cudaSuccess) return c->fail(MRN_ERR_CUDA, "cudaGraphInstantiate: %s", cudaGetErrorString(inst));
+  return MRN_OK;
+}
 
 int get_bucket(mrn_ctx* c, int n, Bucket** out) {
   const int key = bucket_for(n);
@@ -430,20 +452,7 @@ int get_bucket(mrn_ctx* c, int n, Bucket** out) {
   Bucket b;
   b.positions = key;
   int rc = make_plans(c, b);
-  if (rc) return rc;
-  // Capture the forward pass into a graph (src/net/cuda/mod.rs:689-700).
-  CK(cudaStreamBeginCapture(c->stream, cudaStreamCaptureModeThreadLocal));
-  rc = enqueue(c, b, c->stream, nullptr, nullptr);
-  cudaGraph_t graph = nullptr;
-  const cudaError_t end = cudaStreamEndCapture(c->stream, &graph);
-  if (rc) {
-    if (graph) cudaGraphDestroy(graph);
-    return rc;
-  }
-  if (end != cudaSuccess || !graph) return c->fail(MRN_ERR_CUDA, "graph capture failed: %s", cudaGetErrorString(end));
-  const cudaError_t inst = cudaGraphInstantiate(&b.graph, graph, 0);
-  cudaGraphDestroy(graph);
-  if (inst != cudaSuccess) return c->fail(MRN_ERR_CUDA, "cudaGraphInstantiate: %s", cudaGetErrorString(inst));
+  if (rc || (rc = capture(c, b, HeadsOut::kPriors, c->priors, &b.graph))) return rc;
   *out = &c->buckets.emplace(key, std::move(b)).first->second;
   return MRN_OK;
 }
@@ -504,7 +513,10 @@ void destroy(mrn_ctx* c) {
   cudaSetDevice(c->device);
   if (c->stream) cudaStreamSynchronize(c->stream);
   for (auto& kv : c->buckets)
-    if (kv.second.graph) cudaGraphExecDestroy(kv.second.graph);
+    for (cudaGraphExec_t g : {kv.second.graph, kv.second.slot_graph})
+      if (g) cudaGraphExecDestroy(g);
+  if (c->moves_dev) cudaFree(c->moves_dev);
+  if (c->moves_host) cudaFreeHost(c->moves_host);
   for (void* p : c->allocations) cudaFree(p);
   if (c->h_boards) cudaFreeHost(c->h_boards);
   if (c->h_legal) cudaFreeHost(c->h_legal);
@@ -524,6 +536,24 @@ const char* precision_name(int p) {
 }
 
 }  // namespace
+
+namespace mrn {
+
+int slot_logits_bucket(mrn_ctx* c, int n, Bucket** out) {
+  int rc = get_bucket(c, n, out);
+  if (rc) return rc;
+  if (!c->slot_logits &&
+      (rc = dev_alloc(c, &c->slot_logits, static_cast<size_t>(c->max_bucket) * MRN_MAX_LEGAL * 4)))
+    return rc;
+  if (!(*out)->slot_graph) return capture(c, **out, HeadsOut::kSlotLogits, c->slot_logits, &(*out)->slot_graph);
+  return MRN_OK;
+}
+
+int check_boards(mrn_ctx* c, int n, const uint8_t* boards) { return validate_inputs(c, n, boards, nullptr); }
+
+int status_error(mrn_ctx* c, int word) { return check_status(c, word); }
+
+}  // namespace mrn
 
 extern "C" {
 
@@ -714,7 +744,7 @@ MRN_API int mrn_logits(mrn_ctx* c, int n, const uint8_t* boards, float* policy, 
   CK(cudaMemcpyAsync(c->boards, boards, static_cast<size_t>(n) * MRN_BOARD_BYTES, cudaMemcpyHostToDevice, s));
   if (P > n)
     CK(cudaMemsetAsync(c->boards + static_cast<size_t>(n) * MRN_BOARD_BYTES, 0, static_cast<size_t>(P - n) * MRN_BOARD_BYTES, s));
-  if ((rc = enqueue(c, *b, s, c->logits, nullptr))) return rc;
+  if ((rc = enqueue(c, *b, s, HeadsOut::kAllLogits, c->logits, nullptr))) return rc;
   CK(cudaMemcpyAsync(policy, c->logits, static_cast<size_t>(n) * MRN_ACTIONS * 4, cudaMemcpyDeviceToHost, s));
   CK(cudaMemcpyAsync(value, c->wdl, static_cast<size_t>(n) * 3 * 4, cudaMemcpyDeviceToHost, s));
   CK(cudaMemcpyAsync(c->h_status, c->status, 4, cudaMemcpyDeviceToHost, s));
@@ -787,7 +817,7 @@ MRN_API int mrn_profile(mrn_ctx* c, int n, const uint8_t* d_boards, const int32_
   }
   Profiler prof;
   prof.stream = s;
-  rc = enqueue(c, *b, s, nullptr, &prof);
+  rc = enqueue(c, *b, s, HeadsOut::kPriors, c->priors, &prof);
   CK(cudaStreamSynchronize(s));
   for (int i = 0; i < MRN_PROFILE_SLOTS; ++i) times_ms[i] = 0.f, flops[i] = 0.0, launches[i] = 0;
   for (auto& m : prof.marks) {

@@ -33,6 +33,7 @@ struct Bucket {
   int positions = 0;
   std::vector<GemmPlan> plans;  // 4 per layer (QKV, out-proj, FFN1, FFN2), then the value head's first layer
   cudaGraphExec_t graph = nullptr;
+  cudaGraphExec_t slot_graph = nullptr;  // raw logits of the legal slots; captured by the first mrn_evaluate_moves
 };
 
 // Buffers one forward pass runs on (the context's own, or the static scratch's).
@@ -102,6 +103,11 @@ struct mrn_ctx {
   int* status = nullptr;
   float* logits = nullptr;  // [max_bucket, 4672], allocated by the first mrn_logits
   __half* priors16 = nullptr;  // [max_bucket, 224], allocated by the first mrn_evaluate_f16
+  float* slot_logits = nullptr;  // [max_bucket, 224], allocated by the first mrn_evaluate_moves
+  // mrn_evaluate_moves / mrn_choose_moves: the call's lists and rules, and what it returns
+  uint8_t* moves_dev = nullptr;
+  uint8_t* moves_host = nullptr;
+  size_t moves_bytes = 0;
   // pinned staging
   uint8_t* h_boards = nullptr;
   int32_t* h_legal = nullptr;
@@ -141,6 +147,12 @@ namespace mrn {
 // capturer's). After the pass: record its completion on `s`. Both return an mrn_status.
 int begin_pass(mrn_ctx* c, cudaStream_t s);
 int end_pass(mrn_ctx* c, cudaStream_t s);
+// The bucket of a batch of n positions with its pass that leaves the legal slots' raw logits in
+// c->slot_logits (Bucket::slot_graph).
+int slot_logits_bucket(mrn_ctx* c, int n, Bucket** out);
+// The range check of boards, and the mrn_status of a non-zero status word, with their messages.
+int check_boards(mrn_ctx* c, int n, const uint8_t* boards);
+int status_error(mrn_ctx* c, int word);
 // Looks up the static scratch array's device address for c (static_forward.cu); called by
 // mrn_create with c's device current.
 void static_scratch_setup(mrn_ctx* c);

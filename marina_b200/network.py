@@ -140,6 +140,86 @@ class LogitRules(_lib.MrnRules):
 _RULE_PARTS = {name for name, _ in _lib.MrnRules._fields_} - {"actions"}
 
 
+class MoveRules:
+    """`LogitRules` in host memory, for a batch of positions' move lists (`evaluate_moves`,
+    `choose_moves`); every part is optional and an array with one row is shared by the batch:
+
+    * ``mask`` [n or 1, 4672] bool: the actions that may be played;
+    * ``bias`` (actions [n or 1, k], values [n or 1, k]): added to the logits of those actions, -1
+      where a list is shorter;
+    * ``history`` [n or 1, h]: actions played before, -1 where a list is shorter, which ``repetition``,
+      ``presence`` and ``frequency`` (a number, or one per position) make less likely.
+    """
+
+    def __init__(self, mask=None, bias=None, history=None, repetition=None, presence=None, frequency=None):
+        self.mask, self.bias, self.history = mask, bias, history
+        self.penalties = {"repetition": repetition, "presence": presence, "frequency": frequency}
+
+    def packed(self, n: int) -> LogitRules:
+        parts, keep = {}, []
+
+        def rows(name, value, dtype, width=None):
+            a = np.ascontiguousarray(value, dtype=dtype)
+            if a.ndim != 2 or a.shape[0] not in (1, n) or (width is not None and a.shape[1] != width):
+                raise ValueError(f"{name} has shape {list(a.shape)}: expected [{n} or 1, {width or 'entries'}]")
+            return a
+
+        def put(name, a, stride=None):
+            keep.append(a)
+            parts[name] = a.ctypes.data
+            if stride is not None:
+                parts[stride] = 0 if a.shape[0] == 1 else a.shape[1]
+
+        if self.mask is not None:
+            allowed = rows("mask", self.mask, np.bool_, _lib.ACTIONS)
+            put("mask", np.packbits(allowed, axis=1, bitorder="little").view(np.uint32), "mask_stride")
+        if self.bias is not None:
+            ids, values = rows("bias actions", self.bias[0], np.int32), rows("bias values", self.bias[1], np.float32)
+            if ids.shape != values.shape:
+                raise ValueError(f"bias actions {list(ids.shape)} and values {list(values.shape)} differ in shape")
+            if ids.shape[1]:
+                put("bias_actions", ids, "bias_stride")
+                put("bias_values", values)
+                parts["bias_len"] = ids.shape[1]
+        if self.history is not None:
+            played = rows("history", self.history, np.int32)
+            if played.shape[1]:
+                put("history", played, "history_stride")
+                parts["history_len"] = played.shape[1]
+            for name, value in self.penalties.items():
+                if value is not None:
+                    put(name, _per_row(name, value, np.float32, n))
+        rules = LogitRules(_lib.ACTIONS, **parts)
+        rules.arrays = keep
+        return rules
+
+
+def _per_row(name, value, dtype, n: int):
+    """A number, or one per position, as a C array of n; None stays None."""
+    if value is None:
+        return None
+    a = np.asarray(value, dtype=dtype)
+    if a.shape not in ((), (n,)):
+        raise ValueError(f"{name} has shape {list(a.shape)}: expected a number or [{n}]")
+    return np.ascontiguousarray(np.broadcast_to(a, (n,)))
+
+
+def _data(a):
+    return None if a is None else a.ctypes.data
+
+
+def _move_lists(boards, lengths, actions):
+    boards = np.ascontiguousarray(boards, dtype=np.uint8)
+    lengths = np.ascontiguousarray(lengths, dtype=np.int32)
+    actions = np.ascontiguousarray(actions, dtype=np.int32)
+    n = boards.shape[0]
+    if boards.shape != (n, BOARD_BYTES) or lengths.shape != (n,) or actions.ndim != 1:
+        raise ValueError("boards must be [n, 66], lengths [n] and actions one list")
+    if (lengths < 0).any() or int(lengths.sum(dtype=np.int64)) != len(actions):
+        raise ValueError(f"lengths add up to {int(lengths.sum(dtype=np.int64))}, actions hold {len(actions)}")
+    return n, boards, lengths, actions
+
+
 class B200Network(Network):
     """One GPU's evaluator: `CudaNetwork::new(arch, &weights, ordinal, max_batch, fp8)`
     (src/net/cuda/mod.rs:276-493) with `precision` one of "bf16", "fp8w" (e4m3 weights,
@@ -241,6 +321,39 @@ class B200Network(Network):
         rc = self._lib.mrn_evaluate_device_static(self._ctx, n, c_void_p(boards_ptr), c_void_p(legal_ptr),
                                                   c_void_p(priors_ptr), c_void_p(wdl_ptr), c_void_p(stream or 0))
         self._check(rc, "static-scratch forward")
+
+    # -- move lists ---------------------------------------------------------------------------
+    def evaluate_moves(self, boards: np.ndarray, lengths: np.ndarray, actions: np.ndarray,
+                       rules: MoveRules | None = None, temperature=None) -> tuple[np.ndarray, np.ndarray]:
+        """`mrn_evaluate_moves`: boards [n, 66], lengths [n] and the positions' legal actions one list
+        behind the other. Returns a prior for each listed action, in the same order, under `rules` and
+        at `temperature` (a number or one per position), and wdl [n, 3]."""
+        n, boards, lengths, actions = _move_lists(boards, lengths, actions)
+        packed = None if rules is None else rules.packed(n)
+        t = _per_row("temperature", temperature, np.float32, n)
+        priors = np.empty(len(actions), dtype=np.float32)
+        wdl = np.empty((n, 3), dtype=np.float32)
+        rc = self._lib.mrn_evaluate_moves(self._ctx, n, _data(boards), _data(lengths), _data(actions), packed, _data(t),
+                                          _data(priors), _data(wdl))
+        self._check(rc, "forward on move lists")
+        return priors, wdl
+
+    def choose_moves(self, boards: np.ndarray, lengths: np.ndarray, actions: np.ndarray, uniform=None,
+                     rules: MoveRules | None = None, temperature=None, top_k=None,
+                     top_p=None) -> tuple[np.ndarray, np.ndarray, np.ndarray]:
+        """`mrn_choose_moves`: one move per position, drawn with `uniform` (numbers in [0, 1), one per
+        position; None: the likeliest move). Returns the move's place in its position's list (-1: none
+        is left), its probability and wdl [n, 3]."""
+        n, boards, lengths, actions = _move_lists(boards, lengths, actions)
+        packed = None if rules is None else rules.packed(n)
+        t, u = _per_row("temperature", temperature, np.float32, n), _per_row("uniform", uniform, np.float32, n)
+        k, p = _per_row("top_k", top_k, np.int32, n), _per_row("top_p", top_p, np.float32, n)
+        move, prob = np.empty(n, dtype=np.int32), np.empty(n, dtype=np.float32)
+        wdl = np.empty((n, 3), dtype=np.float32)
+        rc = self._lib.mrn_choose_moves(self._ctx, n, _data(boards), _data(lengths), _data(actions), packed, _data(t),
+                                        _data(k), _data(p), _data(u), _data(move), _data(prob), _data(wdl))
+        self._check(rc, "choice of moves")
+        return move, prob, wdl
 
     # -- policy operators (device pointers; enqueued on `stream`, the context's own if None) -----
     def slot_table(self, rows: int, width: int, lengths_ptr: int, count: int, entries_ptr: int, starts_ptr: int,
