@@ -338,27 +338,8 @@ __global__ void __launch_bounds__(kNarrowWarps * 32) adjust_narrow_kernel(Adjust
     if (32 * k + lane < width) priors[32 * k + lane] = e[k];
 }
 
-__device__ __forceinline__ uint64_t warp_sum_u64(uint64_t v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-  return v;
-}
-
-// Exclusive sums over the lanes.
-__device__ __forceinline__ uint64_t warp_exclusive_u64(uint64_t v, int lane) {
-  uint64_t in = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint64_t u = __shfl_up_sync(~0u, in, o);
-    if (lane >= o) in += u;
-  }
-  return in - v;
-}
-
 // Draws from the `left` <= 32 G columns in sh.x, which are in column order. With a cut-off they are
-// sorted by (logit, lower column) in a bitonic network, 32 G elements in the order i = lane G + g:
-// exchanges at a distance below G stay in a thread, the others are shuffles. A weight is computed
-// once for each column.
+// sorted by (logit, lower column), and a weight is computed once for each column.
 template <int G, int K>
 __device__ __forceinline__ Choice draw_narrow(const ChooseParams& p, int row, int lane, NarrowShared<K>& sh, int left,
                                               const Weights& weight) {
@@ -373,32 +354,7 @@ __device__ __forceinline__ Choice draw_narrow(const ChooseParams& p, int row, in
       const int i = lane * G + g;
       e[g] = i < left ? static_cast<uint64_t>(order_key(sh.x[i])) << 32 | ~static_cast<uint32_t>(i) : 0;
     }
-#pragma unroll
-    for (int size = 2; size <= 32 * G; size <<= 1) {
-#pragma unroll
-      for (int d = size >> 1; d; d >>= 1) {
-        if (d >= G) {
-#pragma unroll
-          for (int g = 0; g < G; ++g) {
-            const uint64_t o = __shfl_xor_sync(~0u, e[g], d / G);
-            const int i = lane * G + g;
-            const bool larger = ((i & d) == 0) == ((i & size) == 0 || size == 32 * G);
-            e[g] = (e[g] > o) == larger ? e[g] : o;
-          }
-        } else {
-#pragma unroll
-          for (int g = 0; g < G; ++g)
-            if (!(g & d)) {
-              const int i = lane * G + g;
-              const bool down = (i & size) == 0 || size == 32 * G;
-              const uint64_t x = e[g], y = e[g | d];
-              const bool swap = (x < y) == down;
-              e[g] = swap ? y : x;
-              e[g | d] = swap ? x : y;
-            }
-        }
-      }
-    }
+    warp_sort<G>(e, lane);
     const int most = k > 0 ? min(k, left) : left;
     uint64_t mine = 0;
 #pragma unroll

@@ -65,11 +65,12 @@ struct Weights {
   float m32, inv_t32;
   __device__ __forceinline__ Weights(float max, float t)
       : m(max), inv_t(1.0 / static_cast<double>(t)), infinite(max == INFINITY), m32(max), inv_t32(1.f / t) {}
+  // False only for logits that weigh 0: below -41 ln 2 = -28.42 the weight rounds to 0, and three
+  // roundings in f32 move -28.5 by less than 1e-5.
+  __device__ __forceinline__ bool maybe(float x) const { return !((x - m32) * inv_t32 < -28.5f) && x > -INFINITY; }
   __device__ __forceinline__ uint64_t operator()(float x) const {
-    if (!(x > -INFINITY)) return 0;
+    if (!maybe(x)) return 0;
     if (infinite) return x == INFINITY ? static_cast<uint64_t>(kWeightOne) : 0;
-    // Below -41 ln 2 = -28.42 the weight rounds to 0; three roundings in f32 move -28.5 by less than 1e-5.
-    if ((x - m32) * inv_t32 < -28.5f) return 0;
     return static_cast<uint64_t>(__double2ll_rn(exp((static_cast<double>(x) - m) * inv_t) * kWeightOne));
   }
 };
@@ -83,6 +84,55 @@ __device__ __forceinline__ uint64_t needed_mass(float top_p, uint64_t mass) {
 __device__ __forceinline__ uint64_t drawn_unit(float uniform, uint64_t mass) {
   const double at = static_cast<double>(uniform) * static_cast<double>(mass);
   return at > 0.0 ? min(static_cast<uint64_t>(at), mass - 1) : 0;
+}
+
+__device__ __forceinline__ uint64_t warp_sum_u64(uint64_t v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  return v;
+}
+
+// Exclusive sums over the lanes.
+__device__ __forceinline__ uint64_t warp_exclusive_u64(uint64_t v, int lane) {
+  uint64_t in = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint64_t u = __shfl_up_sync(~0u, in, o);
+    if (lane >= o) in += u;
+  }
+  return in - v;
+}
+
+// Sorts 32 G elements of a warp, largest first, in a bitonic network. Element i is lane i / G's
+// e[i % G]: exchanges at a distance below G stay in a thread, the others are shuffles.
+template <int G>
+__device__ __forceinline__ void warp_sort(uint64_t (&e)[G], int lane) {
+#pragma unroll
+  for (int size = 2; size <= 32 * G; size <<= 1) {
+#pragma unroll
+    for (int d = size >> 1; d; d >>= 1) {
+      if (d >= G) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const uint64_t o = __shfl_xor_sync(~0u, e[g], d / G);
+          const int i = lane * G + g;
+          const bool larger = ((i & d) == 0) == ((i & size) == 0 || size == 32 * G);
+          e[g] = (e[g] > o) == larger ? e[g] : o;
+        }
+      } else {
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+          if (!(g & d)) {
+            const int i = lane * G + g;
+            const bool down = (i & size) == 0 || size == 32 * G;
+            const uint64_t x = e[g], y = e[g | d];
+            const bool swap = (x < y) == down;
+            e[g] = swap ? y : x;
+            e[g | d] = swap ? x : y;
+          }
+      }
+    }
+  }
 }
 
 struct Choice {

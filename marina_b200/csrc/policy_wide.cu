@@ -1,10 +1,10 @@
 // The policy operators on rows of more than kNarrowWidth columns: a cluster of blocks takes a row,
-// each block a contiguous segment of its columns, which it reads once, adjusts, and holds in shared
-// memory until the row is done. Blocks of a row exchange maxima, sums and histograms through
-// distributed shared memory.
+// each block a contiguous segment of its columns, which it reads once into registers. Blocks of a row
+// exchange maxima, sums and histograms through distributed shared memory.
 #include <cooperative_groups.h>
 #include <stdlib.h>
 
+#include <type_traits>
 #include <utility>
 
 #include "kernels.cuh"
@@ -12,6 +12,7 @@
 #include "policy.cuh"
 #include "policy_rows.cuh"
 #include "ptx.cuh"
+#include "rows.cuh"
 
 namespace mrn {
 
@@ -23,11 +24,14 @@ constexpr int kMaxThreads = 512;
 constexpr int kMaxWarps = kMaxThreads / 32;
 constexpr int kMaxBlocks = 8;  // of a cluster; what every device schedules
 constexpr int kMaxSegment = kPolicyMaxWidth / kMaxBlocks;
+constexpr int kQuadsNarrow = 8, kQuadsWide = 16;  // columns a thread holds, over four
+constexpr int blocks_per_sm(int quads) { return quads <= kQuadsNarrow ? 2 : 1; }  // of kMaxThreads: 64 or 128 registers
+constexpr int kSpan = 128;  // columns that a warp takes at a time, four to a lane
 
 // This block's part of its row.
 struct Part {
   int row, rank, blocks;
-  int c0, n;  // columns [c0, c0 + n); c0 is a multiple of 32, n may be 0
+  int c0, n;  // columns [c0, c0 + n); c0 is a multiple of kSpan, n may be 0
 };
 
 __device__ __forceinline__ Part my_part(int blocks, int segment, int width) {
@@ -77,18 +81,74 @@ __device__ __forceinline__ V row_reduce(const Part& q, V v, F f, Exchange<V>& ex
   return v;
 }
 
-// The adjusted logits of the block's columns into x[0, n). Thread t holds the columns t,
-// t + blockDim.x, ... of the segment, and sees only its own until the next barrier.
+// The registers of a row: thread t holds NQ times four columns. Span k of a warp is the block's columns
+// from kSpan * (warp + warps * k) on; with QUADS, where every row starts on a boundary of four elements,
+// lane l holds columns 4 l + j of it, read four at a time; otherwise the columns 32 j + l, each read
+// of the warp one contiguous piece.
+template <bool QUADS>
+__device__ __forceinline__ int span_column(int j) {
+  const int lane = threadIdx.x & 31;
+  return QUADS ? 4 * lane + j : 32 * j + lane;
+}
+
+__device__ __forceinline__ int span_base(int k) {
+  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  return kSpan * (warp + warps * k);
+}
+
 template <class T>
-__device__ __forceinline__ void load_part(const LogitParams& p, const Part& q, float* x) {
+struct Quad {
+  T v[4];
+};
+
+// f(i, j) for the columns i of span k inside the block's part.
+template <bool QUADS, class T>
+__device__ __forceinline__ void load_span(const T* from, int base, int n, float (&x)[4]) {
+  if (QUADS && base + span_column<QUADS>(3) < n) {
+    using Vector = typename std::conditional<sizeof(T) == 4, float4, uint2>::type;
+    const Vector raw = __ldcs(reinterpret_cast<const Vector*>(from + base + span_column<QUADS>(0)));
+    const Quad<T>& q = reinterpret_cast<const Quad<T>&>(raw);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = as_float(q.v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = base + span_column<QUADS>(j);
+      x[j] = i < n ? as_float(from[i]) : -INFINITY;
+    }
+  }
+}
+
+template <bool QUADS, class T>
+__device__ __forceinline__ void store_span(T* to, int base, int n, const float (&x)[4]) {
+  if (QUADS && base + span_column<QUADS>(3) < n) {
+    using Vector = typename std::conditional<sizeof(T) == 4, float4, uint2>::type;
+    Vector raw;
+    Quad<T>& q = reinterpret_cast<Quad<T>&>(raw);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) from_float(x[j], &q.v[j]);
+    *reinterpret_cast<Vector*>(to + base + span_column<QUADS>(0)) = raw;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = base + span_column<QUADS>(j);
+      if (i < n) from_float(x[j], to + i);
+    }
+  }
+}
+
+// The adjusted logits of the block's columns, -inf behind the last. `cells` is shared memory for the
+// segment's columns, needed where the rows have a history or slots.
+template <class T, int NQ, bool QUADS>
+__device__ __forceinline__ void load_part(const LogitParams& p, const Part& q, float* cells, float (&x)[NQ][4]) {
   const RuleParams& r = p.rules;
   const int n = q.n, c0 = q.c0, tid = threadIdx.x, threads = blockDim.x, row = q.row;
   const T* logits = static_cast<const T*>(p.logits) + row * p.stride + c0;
+  const uint32_t* mask = r.mask ? r.mask + row * r.mask_stride : nullptr;
   const Penalties pen = row_penalties(r, row);
   const int32_t* history = r.history + row * r.history_stride;
   const int32_t* ids = r.bias_actions + row * r.bias_stride;
   const float* values = r.bias_values + row * r.bias_stride;
-  const uint32_t* mask = r.mask ? r.mask + row * r.mask_stride : nullptr;
   if (r.columns) {
     // Slots of a wide row: each column counts its action in the history by itself.
     const int32_t* columns = r.columns + row * r.columns_stride + c0;
@@ -103,129 +163,200 @@ __device__ __forceinline__ void load_part(const LogitParams& p, const Part& q, f
         for (int e = 0; e < r.bias_len; ++e)
           if (ids[e] == a) v = __fadd_rn(v, values[e]);
       }
-      x[i] = v;
+      cells[i] = v;
     }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NQ; ++k)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = span_base(k) + span_column<QUADS>(j);
+        x[k][j] = i < n ? cells[i] : -INFINITY;
+      }
+    __syncthreads();
     return;
   }
-  int* counts = reinterpret_cast<int*>(x);  // a cell holds its count until its logit replaces it
+#pragma unroll
+  for (int k = 0; k < NQ; ++k) load_span<QUADS>(logits, span_base(k), n, x[k]);
   if (pen.seen > 0) {
-    for (int i = tid; i < n; i += threads) counts[i] = 0;
+    int* counts = reinterpret_cast<int*>(cells);
+    for (int i = tid; 4 * i < n; i += threads) reinterpret_cast<int4*>(counts)[i] = make_int4(0, 0, 0, 0);
     __syncthreads();
     for (int h = tid; h < pen.seen; h += threads) {
       const int id = history[h];
       if (id >= c0 && id - c0 < n) atomicAdd(&counts[id - c0], 1);
     }
     __syncthreads();
-  }
-  constexpr int kAhead = 8;  // logits in flight per thread
-  for (int i0 = tid; i0 < n; i0 += kAhead * threads) {
-    float v[kAhead];
-    uint32_t word[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int i = i0 + u * threads;
-      v[u] = i < n ? as_float(logits[i]) : 0.f;
-      word[u] = mask && i < n ? mask[(c0 + i) >> 5] : ~0u;
-    }
+    for (int k = 0; k < NQ; ++k) {
+      const int i = span_base(k) + span_column<QUADS>(0);
+      if (QUADS) {
+        if (i < n) {
+          const int4 c = *reinterpret_cast<const int4*>(counts + i);  // a cell behind n holds 0
+          if (c.x | c.y | c.z | c.w) {
+            x[k][0] = penalised(x[k][0], c.x, pen);
+            x[k][1] = penalised(x[k][1], c.y, pen);
+            x[k][2] = penalised(x[k][2], c.z, pen);
+            x[k][3] = penalised(x[k][3], c.w, pen);
+          }
+        }
+      } else {
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int i = i0 + u * threads;
-      if (i < n) {
-        if (pen.seen > 0) v[u] = penalised(v[u], counts[i], pen);
-        x[i] = (word[u] >> ((c0 + i) & 31)) & 1 ? v[u] : -INFINITY;
+        for (int j = 0; j < 4; ++j)
+          if (i + 32 * j < n) x[k][j] = penalised(x[k][j], counts[i + 32 * j], pen);
       }
     }
   }
-  if (r.bias_len) {
-    // A column's entries are all added by the warp that the column belongs to, which goes through the
-    // whole list in its order.
-    __syncthreads();
-    const int lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
-    for (int e0 = 0; e0 < r.bias_len; e0 += 32) {
-      const int id = e0 + lane < r.bias_len ? ids[e0 + lane] : -1;
-      bool mine = id >= c0 && id - c0 < n && (id - c0) % warps == warp;
-      if (mine && mask) mine = (mask[id >> 5] >> (id & 31)) & 1;
-      unsigned todo = __ballot_sync(~0u, mine);
-      while (todo) {
-        const int j = __ffs(todo) - 1;
-        todo &= todo - 1;
-        if (lane == j) x[id - c0] = __fadd_rn(x[id - c0], values[e0 + j]);
-        __syncwarp();
+  if (mask) {
+#pragma unroll
+    for (int k = 0; k < NQ; ++k) {
+      uint32_t word = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = span_base(k) + span_column<QUADS>(j);
+        if (!QUADS || j == 0) word = i < n ? __ldg(mask + ((c0 + i) >> 5)) : 0u;  // four columns of a quad share a word
+        if (!((word >> ((c0 + i) & 31)) & 1)) x[k][j] = -INFINITY;
       }
     }
-    __syncthreads();
+  }
+  // A column's entries are all added by the warp that holds the column, which goes through the whole
+  // list in its order.
+  const int lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
+  for (int e0 = 0; e0 < r.bias_len; e0 += 32) {
+    const int e = e0 + lane;
+    const unsigned i = e < r.bias_len ? static_cast<unsigned>(ids[e]) - static_cast<unsigned>(c0) : ~0u;
+    const int span = static_cast<int>(i / kSpan);
+    bool mine = i < static_cast<unsigned>(n) && span % warps == warp;  // a negative id is far behind n
+    if (mine && mask) mine = (mask[(c0 + i) >> 5] >> ((c0 + i) & 31)) & 1;
+    unsigned todo = __ballot_sync(~0u, mine);
+    if (!todo) continue;
+    const float value = mine ? values[e] : 0.f;
+    const int in = static_cast<int>(i % kSpan);
+    // where the column is: its register, and its lane in the upper bits
+    const int place = 4 * (span / warps) + (QUADS ? in % 4 : in / 32) + ((QUADS ? in / 4 : in % 32) << 16);
+    while (todo) {
+      const int from = __ffs(todo) - 1;
+      todo &= todo - 1;
+      const int to = __shfl_sync(~0u, place, from);
+      const float add = __shfl_sync(~0u, value, from);
+      const int slot = to >> 16 == lane ? to & 0xffff : -1;
+#pragma unroll
+      for (int k = 0; k < NQ; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (slot == 4 * k + j) x[k][j] = __fadd_rn(x[k][j], add);
+    }
   }
 }
 
-// The row's largest logit and its lowest column as (order key, ~column): 0 where nothing is left,
-// all ones where a column that is left holds NaN.
-__device__ __forceinline__ uint64_t row_best(const Part& q, const float* x, Exchange<uint64_t>& ex) {
-  uint64_t best = 0;
-  for (int i = threadIdx.x; i < q.n; i += blockDim.x) {
-    const float v = x[i];
-    uint64_t k = 0;
-    if (v != v) k = ~0ull;
-    else if (v > -INFINITY) k = static_cast<uint64_t>(order_key(v)) << 32 | ~static_cast<uint32_t>(q.c0 + i);
-    if (k > best) best = k;
-  }
-  return row_reduce(q, best, [](uint64_t a, uint64_t b) { return a > b ? a : b; }, ex);
+// The order key of the row's largest logit: 0 where nothing is left, all ones where a column that is
+// left holds NaN.
+template <int NQ>
+__device__ __forceinline__ uint32_t row_best(const Part& q, const float (&x)[NQ][4], Exchange<uint32_t>& ex) {
+  float m = -INFINITY;
+  bool nan = false;
+#pragma unroll
+  for (int k = 0; k < NQ; ++k)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m = fmaxf(m, x[k][j]), nan |= x[k][j] != x[k][j];
+  const uint32_t key = nan ? ~0u : m == -INFINITY ? 0u : order_key(m);
+  return row_reduce(q, key, [](uint32_t a, uint32_t b) { return a > b ? a : b; }, ex);
 }
 
-template <class T>
-__global__ void __launch_bounds__(kMaxThreads) adjust_wide_kernel(AdjustParams p, int blocks, int segment) {
-  extern __shared__ __align__(16) float x[];
-  __shared__ Exchange<uint64_t> ex_best;
+// The lowest column that holds m.
+template <int NQ, bool QUADS>
+__device__ __forceinline__ int row_first(const Part& q, const float (&x)[NQ][4], float m, Exchange<int>& ex) {
+  int first = kPolicyMaxWidth;
+#pragma unroll
+  for (int k = NQ - 1; k >= 0; --k)
+#pragma unroll
+    for (int j = 3; j >= 0; --j)
+      if (x[k][j] == m) first = min(first, q.c0 + span_base(k) + span_column<QUADS>(j));
+  return row_reduce(q, first, [](int a, int b) { return a < b ? a : b; }, ex);
+}
+
+__device__ __forceinline__ float power_of_two(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// Bound by HBM: a logit is read once, stays in a register through maximum, exponential and sum, and
+// leaves as its adjusted value and its prior.
+template <class T, int NQ, bool QUADS>
+__global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(NQ)) adjust_wide_kernel(AdjustParams p, int blocks, int segment) {
+  extern __shared__ __align__(16) float cells[];
+  __shared__ Exchange<uint32_t> ex_best;
+  __shared__ Exchange<int> ex_first;
   __shared__ Exchange<float> ex_sum;
   grid_dep_wait();
   grid_dep_launch();
   const Part q = my_part(blocks, segment, p.in.width);
-  const int tid = threadIdx.x, threads = blockDim.x;
-  load_part<T>(p.in, q, x);
-  T* out = p.out ? static_cast<T*>(p.out) + q.row * p.out_stride + q.c0 : nullptr;
-  if (!p.priors) {
-    for (int i = tid; i < q.n; i += threads) from_float(x[i], out + i);
-    return;
+  float x[NQ][4];
+  load_part<T, NQ, QUADS>(p.in, q, cells, x);
+  if (p.out) {
+    T* out = static_cast<T*>(p.out) + q.row * p.out_stride + q.c0;
+#pragma unroll
+    for (int k = 0; k < NQ; ++k) store_span<QUADS>(out, span_base(k), q.n, x[k]);
   }
-  const uint64_t best = row_best(q, x, ex_best);
+  if (!p.priors) return;
+  const uint32_t best = row_best(q, x, ex_best);
   const float t = p.in.temperature ? p.in.temperature[q.row] : 1.f;
-  const bool nan = best == ~0ull || t != t;
-  const float m = best ? key_value(static_cast<uint32_t>(best >> 32)) : -INFINITY;
+  const float m = key_value(best);
   float sum = 0.f;
-  for (int i = tid; i < q.n; i += threads) {
-    const float v = x[i];
-    if (out) from_float(v, out + i);
-    float e;
-    if (v == -INFINITY) e = 0.f;
-    else if (nan) e = NAN;
-    else if (t <= 0.f) e = static_cast<uint32_t>(q.c0 + i) == ~static_cast<uint32_t>(best) ? 1.f : 0.f;
-    else e = v == m ? 1.f : m == INFINITY ? 0.f : expf((v - m) / t);
-    x[i] = e;
-    sum += e;
+  if (best != ~0u && (t <= 0.f || m == INFINITY)) {
+    // the largest logit's lowest column, or the columns at +inf
+    const int first = t <= 0.f && best ? row_first<NQ, QUADS>(q, x, m, ex_first) : -1;
+#pragma unroll
+    for (int k = 0; k < NQ; ++k)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // (a thread's columns behind the segment, all -inf, are numbered like the next block's)
+        x[k][j] = t <= 0.f ? x[k][j] == m && q.c0 + span_base(k) + span_column<QUADS>(j) == first : t != t && x[k][j] > -INFINITY ? NAN : x[k][j] == m;
+        sum += x[k][j];
+      }
+  } else {
+    // exp((x - m) / t); NaN, in the row or as t, runs through
+    const float top = best ? m : 0.f;
+    const float scale = t != t ? t : fminf(1.44269504088896341f / t, 3.4e38f);  // finite: 0 * scale is 0
+#pragma unroll
+    for (int k = 0; k < NQ; ++k)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[k][j] = x[k][j] == -INFINITY ? 0.f : power_of_two((x[k][j] - top) * scale);
+        sum += x[k][j];
+      }
   }
   sum = row_reduce(q, sum, [](float a, float b) { return a + b; }, ex_sum);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   float* priors = p.priors + q.row * p.priors_stride + q.c0;
-  for (int i = tid; i < q.n; i += threads) {
-    const float e = x[i];
-    priors[i] = e == 0.f ? 0.f : e * inv;  // a masked column's 0 stays one beside a NaN
+#pragma unroll
+  for (int k = 0; k < NQ; ++k) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[k][j] = x[k][j] == 0.f ? 0.f : x[k][j] * inv;  // a masked column stays 0 beside a NaN
+    store_span<QUADS>(priors, span_base(k), q.n, x[k]);
   }
   if (q.blocks > 1) cg::this_cluster().sync();  // no block leaves while another reads from it
 }
 
 // ---- the choice ----------------------------------------------------------------------------
-// Where a row is cut off (top_k, top_p), the last column that is kept is found by its element, (order
-// key of the logit, ~column), so that equal logits are told apart by their columns: a histogram of
-// counts and masses over the distance from the largest logit, kBins bins of 1/36 of a temperature
-// that cover all weights above 0; then the elements of the bin that the border falls into, gathered in
-// one block and sorted. Where a bin holds more than that block's list, the element is found digit by
-// digit instead.
+// Where a row is cut off (top_k, top_p), a histogram over the distance from the largest logit, kBins
+// bins of 1/36 of a temperature that cover all weights above 0, says how far down the border lies.
+// Where no more than kFew columns lie above the end of its bin, they are gathered in the row's first
+// block, and one warp sorts them, cuts them off and draws. Otherwise the last column that is kept is
+// found by its element, (order key of the logit, ~column), so that equal logits are told apart by
+// their columns: among the elements of the border's bin, gathered and sorted, or digit by digit where
+// even the bin holds more than the list; and the draw goes over the whole row again.
 constexpr int kBins = 1024;
 constexpr float kBinsPerUnit = 36.f;  // exp(-1024 / 36) < 2^-41: what lies below weighs 0
+constexpr int kFew = 256;
 
 __host__ __device__ constexpr int list_capacity(int segment) { return segment <= 8192 ? 1024 : 4096; }
 
 struct ChooseShared {
-  Exchange<uint64_t> best, mass_k;
+  Exchange<uint32_t> best;
+  Exchange<int> first;
+  Exchange<uint64_t> mass_k;
   uint64_t warp_sums[kMaxWarps];
   uint64_t scan[kMaxWarps + 1];
   uint64_t digits[256], digit_sums[256];
@@ -233,8 +364,9 @@ struct ChooseShared {
   int digit;
   uint64_t passed;
   // written by the row's first block for the others
+  int border, above;     // the border's bin; columns that lie in it or above
   int bin_k, bin_p;
-  unsigned listed[2];    // elements of bin_k, bin_p
+  unsigned listed[3];    // elements gathered from above the border; from bin_k; from bin_p
   uint64_t before, need; // mass of the bins above bin_p, mass to reach
   uint64_t total_k;
   uint64_t threshold;
@@ -267,6 +399,14 @@ __device__ __forceinline__ uint64_t element(float x, int column) {
   return static_cast<uint64_t>(order_key(x)) << 32 | ~static_cast<uint32_t>(column);
 }
 
+// *cell += w, as two 32-bit additions: shared memory adds those by itself, 64-bit ones in a loop.
+__device__ __forceinline__ void add_mass(uint64_t* cell, uint64_t w) {
+  uint32_t* half = reinterpret_cast<uint32_t*>(cell);
+  const uint32_t low = static_cast<uint32_t>(w), was = atomicAdd(half, low);
+  const uint32_t high = static_cast<uint32_t>(w >> 32) + (was + low < was ? 1u : 0u);
+  if (high) atomicAdd(half + 1, high);
+}
+
 // Exclusive sums over the block's threads; *total: the sum of all.
 __device__ __forceinline__ uint64_t block_exclusive_u64(uint64_t v, ChooseShared& sh, uint64_t* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -292,15 +432,25 @@ __device__ __forceinline__ uint64_t block_exclusive_u64(uint64_t v, ChooseShared
 // one thread calls found(bin, sum of the bins before).
 template <class V, class F>
 __device__ __forceinline__ void find_bin(const V* values, uint64_t need, ChooseShared& sh, F found) {
-  const int per = kBins / blockDim.x, lo = threadIdx.x * per;
+  const int per = (kBins + blockDim.x - 1) / blockDim.x;
+  const int lo = min(static_cast<int>(threadIdx.x) * per, kBins), hi = min(lo + per, kBins);
   uint64_t mine = 0, total;
-  for (int b = lo; b < lo + per; ++b) mine += values[b];
+  for (int b = lo; b < hi; ++b) mine += values[b];
   uint64_t before = block_exclusive_u64(mine, sh, &total);
   if (before < need && need <= before + mine) {
     int b = lo;
     while (before + values[b] < need) before += values[b++];
     found(b, before);
   }
+}
+
+// Sums over the bins below `end`, by one block.
+template <class V>
+__device__ __forceinline__ uint64_t sum_bins(const V* values, int end, ChooseShared& sh) {
+  uint64_t mine = 0, total;
+  for (int b = threadIdx.x; b < end; b += blockDim.x) mine += values[b];
+  block_exclusive_u64(mine, sh, &total);
+  return total;
 }
 
 // Sorts list[0, n), largest first, by one block. The list holds a power of two of at least n.
@@ -333,35 +483,31 @@ struct Border {
     return d < static_cast<float>(kBins) ? static_cast<int>(d) : d != d ? 0 : kBins - 1;  // NaN: inf - inf, 0 * inf
   }
 
-  // f(element, weight) for this block's columns that weigh anything.
+  // f(logit, column of the block) for this block's columns that may weigh anything.
   template <class F>
   __device__ __forceinline__ void each(F f) const {
-    for (int i = threadIdx.x; i < q.n; i += blockDim.x) {
-      const float v = mem.x[i];
-      const uint64_t w = weight(v);
-      if (w) f(v, i, w);
+    for (int i = 4 * threadIdx.x; i < q.n; i += 4 * blockDim.x) {
+      const float4 v = *reinterpret_cast<const float4*>(mem.x + i);  // -inf from n on
+      if (weight.maybe(v.x)) f(v.x, i);
+      if (weight.maybe(v.y)) f(v.y, i + 1);
+      if (weight.maybe(v.z)) f(v.z, i + 2);
+      if (weight.maybe(v.w)) f(v.w, i + 3);
     }
   }
 
-  // The elements of a bin into the first block's list, in any order.
-  __device__ __forceinline__ void gather(int wanted, int which) {
+  // The elements of the bins from `lo` to `hi` into the first block's list, in any order.
+  __device__ __forceinline__ void gather(int lo, int hi, int which) {
     unsigned* listed = at_rank(&sh.listed[which], q, 0);
     uint64_t* list = at_rank(mem.list, q, 0);
-    const int lane = threadIdx.x & 31;
-    for (int i0 = threadIdx.x - lane; i0 < q.n; i0 += blockDim.x) {
-      const int i = i0 + lane;
-      const float v = i < q.n ? mem.x[i] : -INFINITY;
-      const bool in = v > -INFINITY && bin(v) == wanted && weight(v);
-      const unsigned all = __ballot_sync(~0u, in);
-      if (!all) continue;
-      unsigned base = 0;
-      if (lane == 0) base = atomicAdd(listed, static_cast<unsigned>(__popc(all)));
-      base = __shfl_sync(~0u, base, 0) + __popc(all & ((1u << lane) - 1));
-      if (in && base < mem.room) list[base] = element(v, q.c0 + i);
-    }
-  }
-  __device__ __forceinline__ bool fits(int which) const {
-    return *at_rank(&sh.listed[which], q, 0) <= mem.room;
+    each([&](float v, int i) {
+      const int b = bin(v);
+      if (b < lo || b > hi) return;
+      const cg::coalesced_group here = cg::coalesced_threads();
+      unsigned at = 0;
+      if (here.thread_rank() == 0) at = atomicAdd(listed, here.size());
+      at = here.shfl(at, 0) + here.thread_rank();
+      if (at < mem.room) list[at] = element(v, q.c0 + i);
+    });
   }
 
   // The element at which those from `floor` on, largest first, reach `need` in counts or in mass;
@@ -371,11 +517,9 @@ struct Border {
     for (int shift = 56; shift >= 0; shift -= 8) {
       for (int b = threadIdx.x; b < 256; b += blockDim.x) sh.digits[b] = 0;
       __syncthreads();
-      each([&](float v, int i, uint64_t w) {
+      each([&](float v, int i) {
         const uint64_t e = element(v, q.c0 + i);
-        if (e >= floor && (e & known) == prefix)
-          atomicAdd(reinterpret_cast<unsigned long long*>(&sh.digits[(e >> shift) & 255]),
-                    static_cast<unsigned long long>(masses ? w : 1));
+        if (e >= floor && (e & known) == prefix) add_mass(&sh.digits[(e >> shift) & 255], masses ? weight(v) : 1);
       });
       row_sync(q);
       for (int b = threadIdx.x; b < 256; b += blockDim.x) {
@@ -400,59 +544,90 @@ struct Border {
     return prefix;
   }
 
-  // The last element that the row keeps.
-  __device__ uint64_t find(int k, float top_p) {
+  // This block's histogram, added up over the row in the first block.
+  __device__ __forceinline__ void histogram(bool counts, bool masses) {
     const int tid = threadIdx.x, threads = blockDim.x;
-    for (int b = tid; b < kBins; b += threads) mem.masses[b] = 0, mem.counts[b] = 0;
-    if (tid == 0) sh.listed[0] = sh.listed[1] = 0;
+    for (int b = tid; b < kBins; b += threads) {
+      if (counts) mem.counts[b] = 0;
+      if (masses) mem.masses[b] = 0;
+    }
     __syncthreads();
-    each([&](float v, int, uint64_t w) {
+    each([&](float v, int) {
       const int b = bin(v);
-      atomicAdd(reinterpret_cast<unsigned long long*>(&mem.masses[b]), static_cast<unsigned long long>(w));
-      if (k > 0) atomicAdd(&mem.counts[b], 1u);
+      if (counts) atomicAdd(&mem.counts[b], 1u);
+      if (masses) add_mass(&mem.masses[b], weight(v));
     });
     row_sync(q);
-    if (q.blocks > 1) {
-      // each block adds up a share of the bins and hands it to the first
-      const int share = kBins / q.blocks;
-      uint64_t* row_masses = at_rank(mem.row_masses, q, 0);
-      uint32_t* row_counts = at_rank(mem.row_counts, q, 0);
-      for (int b = q.rank * share + tid; b < (q.rank + 1) * share; b += threads) {
-        uint64_t s = 0;
-        uint32_t c = 0;
-        for (int r = 0; r < q.blocks; ++r) s += at_rank(mem.masses, q, r)[b], c += at_rank(mem.counts, q, r)[b];
-        row_masses[b] = s, row_counts[b] = c;
+    if (q.blocks == 1) return;
+    // each block adds up a share of the bins and hands it to the first
+    const int share = kBins / q.blocks;
+    uint64_t* row_masses = at_rank(mem.row_masses, q, 0);
+    uint32_t* row_counts = at_rank(mem.row_counts, q, 0);
+    for (int b = q.rank * share + tid; b < (q.rank + 1) * share; b += threads) {
+      uint64_t s = 0;
+      uint32_t c = 0;
+      for (int r = 0; r < q.blocks; ++r) {
+        if (masses) s += at_rank(mem.masses, q, r)[b];
+        if (counts) c += at_rank(mem.counts, q, r)[b];
       }
-      row_sync(q);
+      if (masses) row_masses[b] = s;
+      if (counts) row_counts[b] = c;
     }
+    row_sync(q);
+  }
+
+  // Histogram and border. True where few columns lie above the border's end, which the first block's
+  // list then holds; sh.total_k is the row's mass where k <= 0.
+  __device__ bool few(int k, float top_p) {
+    if (threadIdx.x == 0) sh.listed[0] = sh.listed[1] = sh.listed[2] = 0, sh.bin_k = -1;
+    histogram(true, k <= 0);
+    if (q.rank == 0) {
+      const uint64_t count = sum_bins(mem.row_counts, kBins, sh);
+      if (k > 0) {
+        if (threadIdx.x == 0) sh.border = kBins - 1, sh.above = static_cast<int>(count);
+        __syncthreads();
+        if (static_cast<uint64_t>(k) < count)
+          find_bin(mem.row_counts, static_cast<uint64_t>(k), sh, [&](int b, uint64_t before) {
+            sh.border = sh.bin_k = b;
+            sh.above = static_cast<int>(before) + static_cast<int>(mem.row_counts[b]);
+            sh.need = static_cast<uint64_t>(k) - before;
+          });
+      } else {
+        const uint64_t total = sum_bins(mem.row_masses, kBins, sh);
+        find_bin(mem.row_masses, needed_mass(top_p, total), sh, [&](int b, uint64_t) { sh.border = b; });
+        __syncthreads();
+        const uint64_t above = sum_bins(mem.row_counts, sh.border + 1, sh);
+        if (threadIdx.x == 0) sh.above = static_cast<int>(above), sh.total_k = total;
+      }
+    }
+    row_sync(q);
+    if (*at_rank(&sh.above, q, 0) > kFew) return false;
+    gather(0, *at_rank(&sh.border, q, 0), 0);
+    row_sync(q);
+    return true;
+  }
+
+  // The last element that the row keeps, after few() said no.
+  __device__ uint64_t find(int k, float top_p) {
+    const int tid = threadIdx.x, threads = blockDim.x;
     const bool lead = q.rank == 0;
     uint64_t floor = 0;
-    int bin_k = -1;
     bool listed = false;  // the first block's list holds bin_k, sorted
-    if (lead) {
-      uint64_t all = 0, mass = 0;
-      for (int b = tid; b < kBins; b += threads) all += mem.row_counts[b], mass += mem.row_masses[b];
-      uint64_t count, total;
-      block_exclusive_u64(all, sh, &count);
-      block_exclusive_u64(mass, sh, &total);
-      if (tid == 0) sh.bin_k = -1, sh.total_k = total;
-      __syncthreads();
-      if (k > 0 && static_cast<uint64_t>(k) < count)
-        find_bin(mem.row_counts, static_cast<uint64_t>(k), sh, [&](int b, uint64_t before) {
-          sh.bin_k = b;
-          sh.need = static_cast<uint64_t>(k) - before;
-        });
-    }
+    const int bin_k = *at_rank(&sh.bin_k, q, 0);
     if (k > 0) {
-      row_sync(q);
-      bin_k = *at_rank(&sh.bin_k, q, 0);
+      histogram(false, true);
+      if (lead) {
+        const uint64_t total = sum_bins(mem.row_masses, kBins, sh);
+        if (tid == 0) sh.total_k = total;
+        __syncthreads();
+      }
       if (bin_k >= 0) {
-        gather(bin_k, 0);
+        gather(bin_k, bin_k, 1);
         row_sync(q);
-        listed = fits(0);
+        listed = *at_rank(&sh.listed[1], q, 0) <= mem.room;
         if (listed) {
           if (lead) {
-            const int n = static_cast<int>(sh.listed[0]), keep = static_cast<int>(sh.need);
+            const int n = static_cast<int>(sh.listed[1]), keep = static_cast<int>(sh.need);
             sort_list(mem.list, n);
             uint64_t mass = 0, total;
             for (int b = tid; b < bin_k; b += threads) mass += mem.row_masses[b];
@@ -465,8 +640,8 @@ struct Border {
         } else {
           floor = by_digits(static_cast<uint64_t>(k), 0, false);
           uint64_t mass = 0;
-          each([&](float v, int i, uint64_t w) {
-            if (element(v, q.c0 + i) >= floor) mass += w;
+          each([&](float v, int i) {
+            if (element(v, q.c0 + i) >= floor) mass += weight(v);
           });
           mass = row_reduce(q, mass, [](uint64_t a, uint64_t b) { return a + b; }, sh.mass_k);
           if (lead && tid == 0) sh.total_k = mass;
@@ -486,15 +661,16 @@ struct Border {
     }
     row_sync(q);
     const int bin_p = *at_rank(&sh.bin_p, q, 0);
-    if (bin_p != bin_k || !listed) {
-      gather(bin_p, 1);
+    const bool again = bin_p != bin_k || !listed;
+    if (again) {
+      gather(bin_p, bin_p, 2);
       row_sync(q);
-      if (!fits(1)) return by_digits(*at_rank(&sh.need, q, 0), floor, true);
-      if (lead) sort_list(mem.list, static_cast<int>(sh.listed[1]));
+      if (*at_rank(&sh.listed[2], q, 0) > mem.room) return by_digits(*at_rank(&sh.need, q, 0), floor, true);
+      if (lead) sort_list(mem.list, static_cast<int>(sh.listed[2]));
     }
     if (lead) {
       __syncthreads();
-      const int n = static_cast<int>(sh.listed[bin_p != bin_k || !listed]);
+      const int n = static_cast<int>(sh.listed[again ? 2 : 1]);
       const int per = (n + threads - 1) / threads, lo = min(tid * per, n), hi = min(lo + per, n);
       uint64_t mine = 0, total;
       for (int i = lo; i < hi; ++i) mine += weight(key_value(static_cast<uint32_t>(mem.list[i] >> 32)));
@@ -513,8 +689,68 @@ struct Border {
   }
 };
 
-template <class T>
-__global__ void __launch_bounds__(kMaxThreads) choose_wide_kernel(ChooseParams p, int blocks, int segment) {
+// Cuts off and draws from the n <= 32 G elements of a list, by one warp; `total` is the row's mass
+// where k <= 0, and `kept` shared memory for 32 G weights.
+template <int G>
+__device__ __forceinline__ Choice draw_few(const uint64_t* list, int n, int k, float top_p, uint64_t total,
+                                           const float* uniform, const Weights& weight, uint64_t* kept) {
+  const int lane = threadIdx.x & 31;
+  uint64_t e[G], w[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) e[g] = lane * G + g < n ? list[lane * G + g] : 0;
+  warp_sort<G>(e, lane);
+  const int most = k > 0 ? min(k, n) : n;
+  uint64_t mine = 0;
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    w[g] = lane * G + g < most ? weight(key_value(static_cast<uint32_t>(e[g] >> 32))) : 0;
+    mine += w[g];
+  }
+  uint64_t ahead = warp_exclusive_u64(mine, lane);
+  if (k > 0) total = __shfl_sync(~0u, ahead + mine, 31);
+  if (top_p < 1.f) {
+    const uint64_t need = needed_mass(top_p, total);
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const uint64_t here = w[g];
+      if (ahead >= need) w[g] = 0;
+      ahead += here;
+    }
+  }
+  // in the order of the columns
+  mine = 0;
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    mine += w[g];
+    kept[lane * G + g] = w[g];
+    e[g] = w[g] ? e[g] << 32 | static_cast<uint32_t>(lane * G + g) : 0;
+  }
+  total = warp_sum_u64(mine);
+  if (!uniform) return Choice{-1, static_cast<float>(kWeightOne / static_cast<double>(total))};  // the largest's
+  const uint64_t unit = drawn_unit(*uniform, total);
+  warp_sort<G>(e, lane);
+  __syncwarp();
+  mine = 0;
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    w[g] = e[g] ? kept[static_cast<uint32_t>(e[g])] : 0;
+    mine += w[g];
+  }
+  ahead = warp_exclusive_u64(mine, lane);
+  int column = -1;
+  uint64_t drawn = 0;
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    if (unit >= ahead && unit < ahead + w[g]) column = static_cast<int>(~static_cast<uint32_t>(e[g] >> 32)), drawn = w[g];
+    ahead += w[g];
+  }
+  const int owner = __ffs(__ballot_sync(~0u, column >= 0)) - 1;
+  return Choice{__shfl_sync(~0u, column, owner),
+                static_cast<float>(static_cast<double>(__shfl_sync(~0u, drawn, owner)) / static_cast<double>(total))};
+}
+
+template <class T, int NQ, bool QUADS>
+__global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(NQ)) choose_wide_kernel(ChooseParams p, int blocks, int segment) {
   extern __shared__ __align__(16) unsigned char dynamic[];
   __shared__ ChooseShared sh;
   grid_dep_wait();
@@ -522,38 +758,61 @@ __global__ void __launch_bounds__(kMaxThreads) choose_wide_kernel(ChooseParams p
   const Part q = my_part(blocks, segment, p.in.width);
   const ChooseMemory mem(dynamic, segment, blocks);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5, row = q.row;
-  load_part<T>(p.in, q, mem.x);
-  const uint64_t best = row_best(q, mem.x, sh.best);
   const float t = p.in.temperature ? p.in.temperature[row] : 1.f;
-  const int first = static_cast<int>(~static_cast<uint32_t>(best));
-  if (best == 0 || best == ~0ull || t != t || t <= 0.f) {
+  uint32_t best;
+  int first = -1;
+  {
+    float x[NQ][4];
+    load_part<T, NQ, QUADS>(p.in, q, mem.x, x);
+    best = row_best(q, x, sh.best);
+    if (best && best != ~0u && (t <= 0.f || !p.uniform)) first = row_first<NQ, QUADS>(q, x, key_value(best), sh.first);
+#pragma unroll
+    for (int k = 0; k < NQ; ++k)
+      if (span_base(k) < segment) store_span<QUADS>(mem.x, span_base(k), segment, x[k]);
+  }
+  if (best == 0 || best == ~0u || !(t > 0.f)) {
     if (q.rank == 0 && tid == 0) {
-      if (best == ~0ull || (best && t != t)) write_choice(p, row, Choice{-1, NAN});
-      else if (best == 0) write_choice(p, row, Choice{-1, t != t ? NAN : 0.f});
-      else write_choice(p, row, Choice{first, 1.f});
+      const bool nan = best == ~0u || t != t;
+      write_choice(p, row, nan ? Choice{-1, NAN} : best ? Choice{first, 1.f} : Choice{-1, 0.f});
     }
-    row_sync(q);
+    row_sync(q);  // no block leaves while another reads from it
     return;
   }
-  const float m = key_value(static_cast<uint32_t>(best >> 32));
+  __syncthreads();
+  const float m = key_value(best);
   const Weights weight(m, t);
   const int k = p.top_k ? p.top_k[row] : 0;
   const float top_p = p.top_p ? p.top_p[row] : 1.f;
   uint64_t last = 0;
-  if (k > 0 || top_p < 1.f) last = Border{q, mem, sh, weight, m, kBinsPerUnit / t}.find(k, top_p);
-  else __syncthreads();  // the draw reads other threads' columns
+  if (k > 0 || top_p < 1.f) {
+    Border border{q, mem, sh, weight, m, kBinsPerUnit / t};
+    if (border.few(k, top_p)) {
+      if (q.rank == 0 && warp == 0) {
+        const int n = static_cast<int>(sh.listed[0]);
+        const float* u = p.uniform ? p.uniform + row : nullptr;
+        Choice c;
+        if (n <= 32) c = draw_few<1>(mem.list, n, k, top_p, sh.total_k, u, weight, sh.digits);
+        else if (n <= 64) c = draw_few<2>(mem.list, n, k, top_p, sh.total_k, u, weight, sh.digits);
+        else if (n <= 128) c = draw_few<4>(mem.list, n, k, top_p, sh.total_k, u, weight, sh.digits);
+        else c = draw_few<8>(mem.list, n, k, top_p, sh.total_k, u, weight, sh.digits);
+        if (!u) c.column = first;
+        if (lane == 0) write_choice(p, row, c);
+      }
+      return;  // the first block reads its own memory only
+    }
+    last = border.find(k, top_p);
+  }
 
   // Column order: each warp takes a run of the block's columns.
   const int run = ((q.n + warps - 1) / warps + 31) & ~31;
   const int lo = min(warp * run, q.n), hi = min(lo + run, q.n);
   auto kept = [&](int i) -> uint64_t {
     const float v = mem.x[i];
-    return v > -INFINITY && element(v, q.c0 + i) >= last ? weight(v) : 0;
+    return weight.maybe(v) && element(v, q.c0 + i) >= last ? weight(v) : 0;
   };
   uint64_t mass = 0;
   for (int i = lo + lane; i < hi; i += 32) mass += kept(i);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) mass += __shfl_xor_sync(~0u, mass, o);
+  mass = warp_sum_u64(mass);
   if (lane == 0) sh.scan[warp] = mass;
   __syncthreads();
   if (tid == 0) {
@@ -582,16 +841,11 @@ __global__ void __launch_bounds__(kMaxThreads) choose_wide_kernel(ChooseParams p
     if (unit >= ahead && unit < end) {
       for (int i0 = lo; i0 < hi; i0 += 32) {
         const uint64_t w = i0 + lane < hi ? kept(i0 + lane) : 0;
-        uint64_t in = w;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint64_t u = __shfl_up_sync(~0u, in, o);
-          if (lane >= o) in += u;
-        }
-        const bool here = w && unit >= ahead + in - w && unit < ahead + in;
+        const uint64_t before = ahead + warp_exclusive_u64(w, lane);
+        const bool here = w && unit >= before && unit < before + w;
         if (here)
           write_choice(p, row, Choice{q.c0 + i0 + lane, static_cast<float>(static_cast<double>(w) / static_cast<double>(total))});
-        ahead += __shfl_sync(~0u, in, 31);
+        ahead = __shfl_sync(~0u, before + w, 31);
         if (__any_sync(~0u, here)) break;
       }
     }
@@ -604,24 +858,46 @@ struct Shape {
 };
 
 // Blocks per row: enough for segments of 8192 columns, and more where the rows alone would leave
-// multiprocessors idle, as long as a segment keeps 1024 columns.
+// multiprocessors idle, as long as a segment keeps 1024 columns. Threads: as many as hold the segment.
 Shape wide_shape(const LogitParams& p) {
-  const int rows = p.rows, width = p.width, sms = p.sms;
+  const int width = p.width;
   int blocks = 1;
-  while (blocks < kMaxBlocks && (width > blocks * 8192 || (static_cast<int64_t>(rows) * blocks < sms && width >= blocks * 2048)))
+  while (blocks < kMaxBlocks &&
+         (width > blocks * 8192 || (static_cast<int64_t>(p.rows) * blocks < p.sms && width >= blocks * 2048)))
     blocks *= 2;
 #ifdef MRN_TUNE
   if (getenv("MRN_B")) blocks = atoi(getenv("MRN_B"));
 #endif
   Shape s;
   s.blocks = blocks;
-  s.segment = ((width + blocks - 1) / blocks + 31) & ~31;
-  s.threads = s.segment <= 2048 ? 256 : 512;
-#ifdef MRN_TUNE
-  if (getenv("MRN_T")) s.threads = atoi(getenv("MRN_T"));
-#endif
+  s.segment = ((width + blocks - 1) / blocks + kSpan - 1) / kSpan * kSpan;
+  const int per_thread = 4 * (s.segment > kMaxThreads * 4 * kQuadsNarrow ? kQuadsWide : kQuadsNarrow);
+  s.threads = (s.segment + 32 * per_thread - 1) / (32 * per_thread) * 32;
+  if (s.threads < 128) s.threads = 128;
   return s;
 }
+
+// f(type, quads per thread, whether they are read at once) for the instantiations. Rows of quads: each
+// row of logits and of the outputs starts on a boundary of four elements.
+template <int N>
+using Int = std::integral_constant<int, N>;
+
+template <class F>
+cudaError_t with_wide(const LogitParams& p, const Shape& shape, bool quads, F&& f) {
+  return with_type(p.type, [&](auto v) {
+    auto with_quads = [&](auto q) {
+      if (shape.segment > kMaxThreads * 4 * kQuadsNarrow) return f(v, Int<kQuadsWide>(), q);
+      return f(v, Int<kQuadsNarrow>(), q);
+    };
+    return quads ? with_quads(std::true_type()) : with_quads(std::false_type());
+  });
+}
+
+bool quad_rows(const void* base, int64_t stride, int size) {
+  return reinterpret_cast<uintptr_t>(base) % (4 * size) == 0 && stride % 4 == 0;
+}
+
+bool quad_rows(const LogitParams& p) { return quad_rows(p.logits, p.stride, p.type == LogitType::kF32 ? 4 : 2); }
 
 template <typename... Params, typename... Args>
 cudaError_t launch_rows(void (*kernel)(Params...), int rows, const Shape& shape, size_t smem, cudaStream_t stream,
@@ -647,8 +923,11 @@ cudaError_t launch_rows(void (*kernel)(Params...), int rows, const Shape& shape,
 
 cudaError_t launch_adjust_wide(const AdjustParams& p, cudaStream_t s) {
   const Shape shape = wide_shape(p.in);
-  return with_type(p.in.type, [&](auto v) {
-    return launch_rows(adjust_wide_kernel<decltype(v)>, p.in.rows, shape, shape.segment * sizeof(float), s, p, shape.blocks,
+  const bool quads = quad_rows(p.in) && (!p.out || quad_rows(p.out, p.out_stride, p.in.type == LogitType::kF32 ? 4 : 2)) &&
+                     (!p.priors || quad_rows(p.priors, p.priors_stride, 4));
+  const size_t smem = p.in.rules.history || p.in.rules.columns ? shape.segment * sizeof(float) : 0;
+  return with_wide(p.in, shape, quads, [&](auto v, auto n, auto q) {
+    return launch_rows(adjust_wide_kernel<decltype(v), n.value, q.value>, p.in.rows, shape, smem, s, p, shape.blocks,
                        shape.segment);
   });
 }
@@ -656,22 +935,29 @@ cudaError_t launch_adjust_wide(const AdjustParams& p, cudaStream_t s) {
 cudaError_t launch_choose_wide(const ChooseParams& p, cudaStream_t s) {
   const Shape shape = wide_shape(p.in);
   const size_t smem = ChooseMemory::bytes(shape.segment, shape.blocks, p.top_k || p.top_p);
-  return with_type(p.in.type, [&](auto v) {
-    return launch_rows(choose_wide_kernel<decltype(v)>, p.in.rows, shape, smem, s, p, shape.blocks, shape.segment);
+  return with_wide(p.in, shape, quad_rows(p.in), [&](auto v, auto n, auto q) {
+    return launch_rows(choose_wide_kernel<decltype(v), n.value, q.value>, p.in.rows, shape, smem, s, p, shape.blocks,
+                       shape.segment);
   });
 }
 
 cudaError_t prepare_policy_wide() {
-  for (LogitType t : {LogitType::kF32, LogitType::kF16, LogitType::kBf16}) {
-    const cudaError_t e = with_type(t, [&](auto v) {
-      const cudaError_t r = cudaFuncSetAttribute(adjust_wide_kernel<decltype(v)>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 static_cast<int>(kMaxSegment * sizeof(float)));
-      if (r != cudaSuccess) return r;
-      return cudaFuncSetAttribute(choose_wide_kernel<decltype(v)>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  static_cast<int>(ChooseMemory::bytes(kMaxSegment, kMaxBlocks, true)));
-    });
-    if (e != cudaSuccess) return e;
-  }
+  for (LogitType t : {LogitType::kF32, LogitType::kF16, LogitType::kBf16})
+    for (int segment : {kMaxThreads * 4 * kQuadsNarrow, kMaxSegment})
+      for (bool quads : {false, true}) {
+        LogitParams in{};
+        in.type = t;
+        const cudaError_t e = with_wide(in, Shape{1, segment, 0}, quads, [&](auto v, auto n, auto q) {
+          const cudaError_t r =
+              cudaFuncSetAttribute(adjust_wide_kernel<decltype(v), n.value, q.value>,
+                                   cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(segment * sizeof(float)));
+          if (r != cudaSuccess) return r;
+          return cudaFuncSetAttribute(choose_wide_kernel<decltype(v), n.value, q.value>,
+                                      cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      static_cast<int>(ChooseMemory::bytes(segment, kMaxBlocks, true)));
+        });
+        if (e != cudaSuccess) return e;
+      }
   return cudaSuccess;
 }
 
