@@ -20,12 +20,12 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kMaxThreads = 512;
+constexpr int kMaxThreads = 1024;
 constexpr int kMaxWarps = kMaxThreads / 32;
 constexpr int kMaxBlocks = 8;  // of a cluster; what every device schedules
 constexpr int kMaxSegment = kPolicyMaxWidth / kMaxBlocks;
-constexpr int kQuadsNarrow = 8, kQuadsWide = 16;  // columns a thread holds, over four
-constexpr int blocks_per_sm(int quads) { return quads <= kQuadsNarrow ? 2 : 1; }  // of kMaxThreads: 64 or 128 registers
+constexpr int kQuads = 8;  // columns a thread holds, over four
+constexpr int kListed = 512;  // entries of a bias list held at a time
 constexpr int kSpan = 128;  // columns that a warp takes at a time, four to a lane
 
 // This block's part of its row.
@@ -81,7 +81,7 @@ __device__ __forceinline__ V row_reduce(const Part& q, V v, F f, Exchange<V>& ex
   return v;
 }
 
-// The registers of a row: thread t holds NQ times four columns. Span k of a warp is the block's columns
+// The registers of a row: thread t holds kQuads times four columns. Span k of a warp is the block's columns
 // from kSpan * (warp + warps * k) on; with QUADS, where every row starts on a boundary of four elements,
 // lane l holds columns 4 l + j of it, read four at a time; otherwise the columns 32 j + l, each read
 // of the warp one contiguous piece.
@@ -139,8 +139,8 @@ __device__ __forceinline__ void store_span(T* to, int base, int n, const float (
 
 // The adjusted logits of the block's columns, -inf behind the last. `cells` is shared memory for the
 // segment's columns, needed where the rows have a history or slots.
-template <class T, int NQ, bool QUADS>
-__device__ __forceinline__ void load_part(const LogitParams& p, const Part& q, float* cells, float (&x)[NQ][4]) {
+template <class T, bool QUADS>
+__device__ __forceinline__ void load_part(const LogitParams& p, const Part& q, float* cells, float (&x)[kQuads][4]) {
   const RuleParams& r = p.rules;
   const int n = q.n, c0 = q.c0, tid = threadIdx.x, threads = blockDim.x, row = q.row;
   const T* logits = static_cast<const T*>(p.logits) + row * p.stride + c0;
@@ -167,7 +167,7 @@ __device__ __forceinline__ void load_part(const LogitParams& p, const Part& q, f
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < NQ; ++k)
+    for (int k = 0; k < kQuads; ++k)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int i = span_base(k) + span_column<QUADS>(j);
@@ -176,19 +176,39 @@ __device__ __forceinline__ void load_part(const LogitParams& p, const Part& q, f
     __syncthreads();
     return;
   }
+  // Everything that the row reads first is asked for at once: the history's first entries, whether the
+  // row has that many or not, the logits, the first of the bias list, and the mask, of which lane
+  // 4 k + j keeps the word for columns 32 j .. 32 j + 31 of span k.
+  const int lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
+  int* counts = reinterpret_cast<int*>(cells);
+  constexpr int kAhead = 2;  // history entries of a thread
+  int seen[kAhead];
 #pragma unroll
-  for (int k = 0; k < NQ; ++k) load_span<QUADS>(logits, span_base(k), n, x[k]);
-  if (pen.seen > 0) {
-    int* counts = reinterpret_cast<int*>(cells);
+  for (int u = 0; u < kAhead; ++u) seen[u] = r.history && tid + u * threads < r.history_len ? history[tid + u * threads] : -1;
+#pragma unroll
+  for (int k = 0; k < kQuads; ++k) load_span<QUADS>(logits, span_base(k), n, x[k]);
+  const int biased = lane < r.bias_len ? ids[lane] : -1;
+  uint32_t words = ~0u;
+  if (mask) {
+    const int i = kSpan * (warp + warps * (lane >> 2)) + 32 * (lane & 3);
+    words = i < n ? __ldg(mask + ((c0 + i) >> 5)) : 0u;
+  }
+  if (r.history) {
     for (int i = tid; 4 * i < n; i += threads) reinterpret_cast<int4*>(counts)[i] = make_int4(0, 0, 0, 0);
     __syncthreads();
-    for (int h = tid; h < pen.seen; h += threads) {
-      const int id = history[h];
-      if (id >= c0 && id - c0 < n) atomicAdd(&counts[id - c0], 1);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (seen[u] >= c0 && seen[u] - c0 < n && tid + u * threads < pen.seen) atomicAdd(&counts[seen[u] - c0], 1);
+    for (int h0 = tid + kAhead * threads; h0 < pen.seen; h0 += kAhead * threads) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) seen[u] = h0 + u * threads < pen.seen ? history[h0 + u * threads] : -1;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (seen[u] >= c0 && seen[u] - c0 < n) atomicAdd(&counts[seen[u] - c0], 1);
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < NQ; ++k) {
+    for (int k = 0; k < kQuads; ++k) {
       const int i = span_base(k) + span_column<QUADS>(0);
       if (QUADS) {
         if (i < n) {
@@ -209,27 +229,24 @@ __device__ __forceinline__ void load_part(const LogitParams& p, const Part& q, f
   }
   if (mask) {
 #pragma unroll
-    for (int k = 0; k < NQ; ++k) {
-      uint32_t word = 0;
+    for (int k = 0; k < kQuads; ++k) {
+      uint32_t word = QUADS ? __shfl_sync(~0u, words, 4 * k + (lane >> 3)) : 0u;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int i = span_base(k) + span_column<QUADS>(j);
-        if (!QUADS || j == 0) word = i < n ? __ldg(mask + ((c0 + i) >> 5)) : 0u;  // four columns of a quad share a word
-        if (!((word >> ((c0 + i) & 31)) & 1)) x[k][j] = -INFINITY;
+        if (!QUADS) word = __shfl_sync(~0u, words, 4 * k + j);
+        if (!((word >> (span_column<QUADS>(j) & 31)) & 1)) x[k][j] = -INFINITY;
       }
     }
   }
-  // A column's entries are all added by the warp that holds the column, which goes through the whole
-  // list in its order.
-  const int lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
-  for (int e0 = 0; e0 < r.bias_len; e0 += 32) {
-    const int e = e0 + lane;
-    const unsigned i = e < r.bias_len ? static_cast<unsigned>(ids[e]) - static_cast<unsigned>(c0) : ~0u;
+  // A column's bias entries are all added by the warp that holds the column, which goes through the
+  // whole list in its order, 32 entries at a time.
+  auto add_listed = [&](unsigned id, int e) {
+    const unsigned i = id - static_cast<unsigned>(c0);  // a negative id is far behind n
     const int span = static_cast<int>(i / kSpan);
-    bool mine = i < static_cast<unsigned>(n) && span % warps == warp;  // a negative id is far behind n
+    bool mine = i < static_cast<unsigned>(n) && span % warps == warp;
     if (mine && mask) mine = (mask[(c0 + i) >> 5] >> ((c0 + i) & 31)) & 1;
     unsigned todo = __ballot_sync(~0u, mine);
-    if (!todo) continue;
+    if (!todo) return;
     const float value = mine ? values[e] : 0.f;
     const int in = static_cast<int>(i % kSpan);
     // where the column is: its register, and its lane in the upper bits
@@ -241,22 +258,34 @@ __device__ __forceinline__ void load_part(const LogitParams& p, const Part& q, f
       const float add = __shfl_sync(~0u, value, from);
       const int slot = to >> 16 == lane ? to & 0xffff : -1;
 #pragma unroll
-      for (int k = 0; k < NQ; ++k)
+      for (int k = 0; k < kQuads; ++k)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (slot == 4 * k + j) x[k][j] = __fadd_rn(x[k][j], add);
     }
+  };
+  if (r.bias_len <= 32) {
+    if (r.bias_len) add_listed(static_cast<unsigned>(biased), lane);
+    return;
+  }
+  __shared__ int listed[kListed];
+  for (int l0 = 0; l0 < r.bias_len; l0 += kListed) {
+    const int length = min(kListed, r.bias_len - l0);
+    __syncthreads();
+    for (int e = tid; e < length; e += threads) listed[e] = ids[l0 + e];
+    __syncthreads();
+#pragma unroll 1
+    for (int e = lane; e - lane < length; e += 32) add_listed(e < length ? static_cast<unsigned>(listed[e]) : ~0u, l0 + e);
   }
 }
 
 // The order key of the row's largest logit: 0 where nothing is left, all ones where a column that is
 // left holds NaN.
-template <int NQ>
-__device__ __forceinline__ uint32_t row_best(const Part& q, const float (&x)[NQ][4], Exchange<uint32_t>& ex) {
-  float m = -INFINITY;
+__device__ __forceinline__ uint32_t row_best(const Part& q, const float (&x)[kQuads][4], Exchange<uint32_t>& ex, float& m) {
+  m = -INFINITY;  // of this thread
   bool nan = false;
 #pragma unroll
-  for (int k = 0; k < NQ; ++k)
+  for (int k = 0; k < kQuads; ++k)
 #pragma unroll
     for (int j = 0; j < 4; ++j) m = fmaxf(m, x[k][j]), nan |= x[k][j] != x[k][j];
   const uint32_t key = nan ? ~0u : m == -INFINITY ? 0u : order_key(m);
@@ -264,11 +293,11 @@ __device__ __forceinline__ uint32_t row_best(const Part& q, const float (&x)[NQ]
 }
 
 // The lowest column that holds m.
-template <int NQ, bool QUADS>
-__device__ __forceinline__ int row_first(const Part& q, const float (&x)[NQ][4], float m, Exchange<int>& ex) {
+template <bool QUADS>
+__device__ __forceinline__ int row_first(const Part& q, const float (&x)[kQuads][4], float m, Exchange<int>& ex) {
   int first = kPolicyMaxWidth;
 #pragma unroll
-  for (int k = NQ - 1; k >= 0; --k)
+  for (int k = kQuads - 1; k >= 0; --k)
 #pragma unroll
     for (int j = 3; j >= 0; --j)
       if (x[k][j] == m) first = min(first, q.c0 + span_base(k) + span_column<QUADS>(j));
@@ -283,8 +312,8 @@ __device__ __forceinline__ float power_of_two(float v) {
 
 // Bound by HBM: a logit is read once, stays in a register through maximum, exponential and sum, and
 // leaves as its adjusted value and its prior.
-template <class T, int NQ, bool QUADS>
-__global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(NQ)) adjust_wide_kernel(AdjustParams p, int blocks, int segment) {
+template <class T, bool QUADS>
+__global__ void __launch_bounds__(kMaxThreads) adjust_wide_kernel(AdjustParams p, int blocks, int segment) {
   extern __shared__ __align__(16) float cells[];
   __shared__ Exchange<uint32_t> ex_best;
   __shared__ Exchange<int> ex_first;
@@ -292,23 +321,24 @@ __global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(NQ)) adjust_wide_ke
   grid_dep_wait();
   grid_dep_launch();
   const Part q = my_part(blocks, segment, p.in.width);
-  float x[NQ][4];
-  load_part<T, NQ, QUADS>(p.in, q, cells, x);
+  float x[kQuads][4];
+  load_part<T, QUADS>(p.in, q, cells, x);
   if (p.out) {
     T* out = static_cast<T*>(p.out) + q.row * p.out_stride + q.c0;
 #pragma unroll
-    for (int k = 0; k < NQ; ++k) store_span<QUADS>(out, span_base(k), q.n, x[k]);
+    for (int k = 0; k < kQuads; ++k) store_span<QUADS>(out, span_base(k), q.n, x[k]);
   }
   if (!p.priors) return;
-  const uint32_t best = row_best(q, x, ex_best);
   const float t = p.in.temperature ? p.in.temperature[q.row] : 1.f;
+  float mine;
+  const uint32_t best = row_best(q, x, ex_best, mine);
   const float m = key_value(best);
   float sum = 0.f;
   if (best != ~0u && (t <= 0.f || m == INFINITY)) {
     // the largest logit's lowest column, or the columns at +inf
-    const int first = t <= 0.f && best ? row_first<NQ, QUADS>(q, x, m, ex_first) : -1;
+    const int first = t <= 0.f && best ? row_first<QUADS>(q, x, m, ex_first) : -1;
 #pragma unroll
-    for (int k = 0; k < NQ; ++k)
+    for (int k = 0; k < kQuads; ++k)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         // (a thread's columns behind the segment, all -inf, are numbered like the next block's)
@@ -320,7 +350,7 @@ __global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(NQ)) adjust_wide_ke
     const float top = best ? m : 0.f;
     const float scale = t != t ? t : fminf(1.44269504088896341f / t, 3.4e38f);  // finite: 0 * scale is 0
 #pragma unroll
-    for (int k = 0; k < NQ; ++k)
+    for (int k = 0; k < kQuads; ++k)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         x[k][j] = x[k][j] == -INFINITY ? 0.f : power_of_two((x[k][j] - top) * scale);
@@ -331,7 +361,7 @@ __global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(NQ)) adjust_wide_ke
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   float* priors = p.priors + q.row * p.priors_stride + q.c0;
 #pragma unroll
-  for (int k = 0; k < NQ; ++k) {
+  for (int k = 0; k < kQuads; ++k) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[k][j] = x[k][j] == 0.f ? 0.f : x[k][j] * inv;  // a masked column stays 0 beside a NaN
     store_span<QUADS>(priors, span_base(k), q.n, x[k]);
@@ -341,19 +371,22 @@ __global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(NQ)) adjust_wide_ke
 
 // ---- the choice ----------------------------------------------------------------------------
 // Where a row is cut off (top_k, top_p), a histogram over the distance from the largest logit, kBins
-// bins of 1/36 of a temperature that cover all weights above 0, says how far down the border lies.
+// bins of 1/18 of a temperature that cover all weights above 0, says how far down the border lies.
 // Where no more than kFew columns lie above the end of its bin, they are gathered in the row's first
-// block, and one warp sorts them, cuts them off and draws. Otherwise the last column that is kept is
+// block, and one warp sorts them, cuts them off and draws: for a small top_k the histogram counts each
+// thread's largest logit only, which puts the border a little too low. Otherwise the last column that is kept is
 // found by its element, (order key of the logit, ~column), so that equal logits are told apart by
 // their columns: among the elements of the border's bin, gathered and sorted, or digit by digit where
 // even the bin holds more than the list; and the draw goes over the whole row again.
-constexpr int kBins = 1024;
-constexpr float kBinsPerUnit = 36.f;  // exp(-1024 / 36) < 2^-41: what lies below weighs 0
+constexpr int kBins = 512;
+constexpr float kBinsPerUnit = 18.f;  // exp(-512 / 18) < 2^-41: what lies below weighs 0
 constexpr int kFew = 256;
 
 __host__ __device__ constexpr int list_capacity(int segment) { return segment <= 8192 ? 1024 : 4096; }
 
 struct ChooseShared {
+  double powers[32];  // 2^(i / 32)
+  int spans[kMaxSegment / kSpan + 1];  // columns that may weigh anything before each span
   Exchange<uint32_t> best;
   Exchange<int> first;
   Exchange<uint64_t> mass_k;
@@ -366,7 +399,7 @@ struct ChooseShared {
   // written by the row's first block for the others
   int border, above;     // the border's bin; columns that lie in it or above
   int bin_k, bin_p;
-  unsigned listed[3];    // elements gathered from above the border; from bin_k; from bin_p
+  unsigned listed[4];    // elements gathered from above the border; from bin_k; from bin_p; from above few_k()'s border
   uint64_t before, need; // mass of the bins above bin_p, mass to reach
   uint64_t total_k;
   uint64_t threshold;
@@ -376,13 +409,16 @@ struct ChooseShared {
 // histogram and the row's (the same memory where a block has the row to itself).
 struct ChooseMemory {
   float* x;
+  uint16_t* places;  // of the columns that may weigh anything, in their order, if they are half the segment or fewer
   uint64_t *list, *masses, *row_masses;
   uint32_t *counts, *row_counts;
   unsigned room;  // elements that the list holds
+  int left;       // places, -1 where there were too many
   __device__ ChooseMemory(unsigned char* base, int segment, int blocks) {
     room = list_capacity(segment);
     x = reinterpret_cast<float*>(base);
-    list = reinterpret_cast<uint64_t*>(x + segment);
+    places = reinterpret_cast<uint16_t*>(x + segment);
+    list = reinterpret_cast<uint64_t*>(places + segment / 2);
     masses = list + room;
     row_masses = blocks > 1 ? masses + kBins : masses;
     counts = reinterpret_cast<uint32_t*>(row_masses + kBins);
@@ -390,8 +426,33 @@ struct ChooseMemory {
   }
   static size_t bytes(int segment, int blocks, bool cut) {
     const size_t histogram = kBins * (sizeof(uint64_t) + sizeof(uint32_t));
-    return segment * sizeof(float) +
+    return segment * sizeof(float) + segment / 2 * sizeof(uint16_t) +
            (cut ? list_capacity(segment) * sizeof(uint64_t) + histogram * (blocks > 1 ? 2 : 1) : 0);
+  }
+};
+
+// Weights (policy_rows.cuh) by a table: with 32 z log2(e) = n + f, n whole and |f| <= 1/2, exp(z) is
+// 2^(n / 32) exp(f ln 2 / 32), the first factor 2^(n >> 5) times one of 32 values, the second the first
+// six terms of its series, the next one below 3e-15. About 15 operations in f64 where exp() takes
+// several times as many: a wide row's f64 pipe is what these kernels run out of first.
+struct TableWeights : Weights {
+  double steps;  // 32 log2(e) / t
+  const double* table;
+  __device__ __forceinline__ TableWeights(float max, float t, const double* powers)
+      : Weights(max, t), steps(46.166241308446828 * inv_t), table(powers) {}
+  __device__ __forceinline__ uint64_t operator()(float x) const {
+    if (!maybe(x)) return 0;
+    if (infinite) return x == INFINITY ? static_cast<uint64_t>(kWeightOne) : 0;
+    constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
+    const double y = (static_cast<double>(x) - m) * steps;
+    const double rounded = y + kRound;
+    const int n = __double2loint(rounded);
+    const double u = (y - (rounded - kRound)) * 0.021660849392498290;  // ln 2 / 32
+    const double series = 1.0 + u * (1.0 + u * (0.5 + u * (1.0 / 6 + u * (1.0 / 24 + u * (1.0 / 120)))));
+    const double power = table[n & 31];  // times 2^(40 + (n >> 5)), through its exponent
+    const double scaled = __hiloint2double(__double2hiint(power) + ((40 + (n >> 5)) << 20), __double2loint(power));
+    constexpr double kWhole = 4503599627370496.0;  // 2^52: the sum's low bits are the rounded product
+    return static_cast<uint64_t>(__double_as_longlong(scaled * series + kWhole)) & ((1ull << 52) - 1);
   }
 };
 
@@ -428,29 +489,33 @@ __device__ __forceinline__ uint64_t block_exclusive_u64(uint64_t v, ChooseShared
   return before + in - v;
 }
 
-// The bin at which the sums of `values` from bin 0 on reach `need` (<= their total), by one block:
-// one thread calls found(bin, sum of the bins before).
-template <class V, class F>
-__device__ __forceinline__ void find_bin(const V* values, uint64_t need, ChooseShared& sh, F found) {
-  const int per = (kBins + blockDim.x - 1) / blockDim.x;
-  const int lo = min(static_cast<int>(threadIdx.x) * per, kBins), hi = min(lo + per, kBins);
-  uint64_t mine = 0, total;
-  for (int b = lo; b < hi; ++b) mine += values[b];
-  uint64_t before = block_exclusive_u64(mine, sh, &total);
-  if (before < need && need <= before + mine) {
-    int b = lo;
-    while (before + values[b] < need) before += values[b++];
-    found(b, before);
-  }
+// Sum of bins [0, end), by one warp.
+template <class V>
+__device__ __forceinline__ uint64_t sum_bins(const V* values, int end) {
+  uint64_t sum = 0;
+  for (int b = threadIdx.x & 31; b < end; b += 32) sum += values[b];
+  return warp_sum_u64(sum);
 }
 
-// Sums over the bins below `end`, by one block.
+// The bin at which the sums of `values` from bin 0 on reach `need`, and the sum of the bins before it,
+// by one warp; -1, and the sum of all, where they never do.
 template <class V>
-__device__ __forceinline__ uint64_t sum_bins(const V* values, int end, ChooseShared& sh) {
-  uint64_t mine = 0, total;
-  for (int b = threadIdx.x; b < end; b += blockDim.x) mine += values[b];
-  block_exclusive_u64(mine, sh, &total);
-  return total;
+__device__ __forceinline__ int find_bin(const V* values, uint64_t need, uint64_t* before) {
+  const int lane = threadIdx.x & 31;
+  uint64_t ahead = 0;
+  for (int b0 = 0; b0 < kBins; b0 += 32) {
+    const uint64_t v = values[b0 + lane];
+    const uint64_t mine = ahead + warp_exclusive_u64(v, lane);
+    const unsigned reached = __ballot_sync(~0u, mine + v >= need);
+    if (reached) {
+      const int first = __ffs(reached) - 1;
+      *before = __shfl_sync(~0u, mine, first);
+      return b0 + first;
+    }
+    ahead = __shfl_sync(~0u, mine + v, 31);
+  }
+  *before = ahead;
+  return -1;
 }
 
 // Sorts list[0, n), largest first, by one block. The list holds a power of two of at least n.
@@ -475,7 +540,7 @@ struct Border {
   const Part& q;
   const ChooseMemory& mem;
   ChooseShared& sh;
-  const Weights& weight;
+  const TableWeights& weight;
   float m, per_bin;
 
   __device__ __forceinline__ int bin(float x) const {
@@ -486,6 +551,10 @@ struct Border {
   // f(logit, column of the block) for this block's columns that may weigh anything.
   template <class F>
   __device__ __forceinline__ void each(F f) const {
+    if (mem.left >= 0) {
+      for (int u = threadIdx.x; u < mem.left; u += blockDim.x) f(mem.x[mem.places[u]], mem.places[u]);
+      return;
+    }
     for (int i = 4 * threadIdx.x; i < q.n; i += 4 * blockDim.x) {
       const float4 v = *reinterpret_cast<const float4*>(mem.x + i);  // -inf from n on
       if (weight.maybe(v.x)) f(v.x, i);
@@ -499,15 +568,29 @@ struct Border {
   __device__ __forceinline__ void gather(int lo, int hi, int which) {
     unsigned* listed = at_rank(&sh.listed[which], q, 0);
     uint64_t* list = at_rank(mem.list, q, 0);
-    each([&](float v, int i) {
+    // Most columns lie below the bins by any rounding.
+    const float low = hi == kBins - 1 ? -INFINITY : m - (static_cast<float>(hi + 1) / per_bin) * 1.0001f - fabsf(m) * 1e-6f;
+    auto add = [&](float v, int i) {
       const int b = bin(v);
-      if (b < lo || b > hi) return;
+      if (b < lo || b > hi || !weight.maybe(v)) return;
       const cg::coalesced_group here = cg::coalesced_threads();
       unsigned at = 0;
       if (here.thread_rank() == 0) at = atomicAdd(listed, here.size());
       at = here.shfl(at, 0) + here.thread_rank();
       if (at < mem.room) list[at] = element(v, q.c0 + i);
-    });
+    };
+    if (mem.left >= 0) {
+      for (int u = threadIdx.x; u < mem.left; u += blockDim.x) add(mem.x[mem.places[u]], mem.places[u]);
+      return;
+    }
+    for (int i = 4 * threadIdx.x; i < q.n; i += 4 * blockDim.x) {
+      const float4 v = *reinterpret_cast<const float4*>(mem.x + i);
+      if (fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) < low) continue;
+      add(v.x, i);
+      add(v.y, i + 1);
+      add(v.z, i + 2);
+      add(v.w, i + 3);
+    }
   }
 
   // The element at which those from `floor` on, largest first, reach `need` in counts or in mass;
@@ -544,26 +627,15 @@ struct Border {
     return prefix;
   }
 
-  // This block's histogram, added up over the row in the first block.
-  __device__ __forceinline__ void histogram(bool counts, bool masses) {
-    const int tid = threadIdx.x, threads = blockDim.x;
-    for (int b = tid; b < kBins; b += threads) {
-      if (counts) mem.counts[b] = 0;
-      if (masses) mem.masses[b] = 0;
-    }
-    __syncthreads();
-    each([&](float v, int) {
-      const int b = bin(v);
-      if (counts) atomicAdd(&mem.counts[b], 1u);
-      if (masses) add_mass(&mem.masses[b], weight(v));
-    });
+  // The blocks' histograms added up over the row, in the first block.
+  __device__ __forceinline__ void add_up(bool counts, bool masses) const {
     row_sync(q);
     if (q.blocks == 1) return;
     // each block adds up a share of the bins and hands it to the first
     const int share = kBins / q.blocks;
     uint64_t* row_masses = at_rank(mem.row_masses, q, 0);
     uint32_t* row_counts = at_rank(mem.row_counts, q, 0);
-    for (int b = q.rank * share + tid; b < (q.rank + 1) * share; b += threads) {
+    for (int b = q.rank * share + threadIdx.x; b < (q.rank + 1) * share; b += blockDim.x) {
       uint64_t s = 0;
       uint32_t c = 0;
       for (int r = 0; r < q.blocks; ++r) {
@@ -576,28 +648,65 @@ struct Border {
     row_sync(q);
   }
 
+  __device__ __forceinline__ void clear(bool counts, bool masses) const {
+    for (int b = threadIdx.x; b < kBins; b += blockDim.x) {
+      if (counts) mem.counts[b] = 0;
+      if (masses) mem.masses[b] = 0;
+    }
+    __syncthreads();
+  }
+
+  __device__ __forceinline__ void histogram(bool counts, bool masses) const {
+    clear(counts, masses);
+    each([&](float v, int) {
+      const int b = bin(v);
+      if (counts) atomicAdd(&mem.counts[b], 1u);
+      if (masses) add_mass(&mem.masses[b], weight(v));
+    });
+    add_up(counts, masses);
+  }
+
+  // Whether no more than kFew columns lie above the end of the border's bin for a small k; the first
+  // block's list then holds them. `mine` is the thread's largest logit: k of the row's threads have one
+  // above the border, so that k of its columns lie there.
+  __device__ __forceinline__ bool few_k(float mine, int k) {
+    if (k > kFew / 2 || 2 * k > static_cast<int>(blockDim.x) * q.blocks) return false;
+    clear(true, false);
+    if (weight.maybe(mine)) atomicAdd(&mem.counts[bin(mine)], 1u);
+    add_up(true, false);
+    if (q.rank == 0 && threadIdx.x < 32) {
+      uint64_t before;
+      const int b = find_bin(mem.row_counts, static_cast<uint64_t>(k), &before);
+      if (threadIdx.x == 0) sh.border = b < 0 ? kBins - 1 : b;
+    }
+    row_sync(q);
+    gather(0, *at_rank(&sh.border, q, 0), 3);
+    row_sync(q);
+    return *at_rank(&sh.listed[3], q, 0) <= kFew;
+  }
+
   // Histogram and border. True where few columns lie above the border's end, which the first block's
   // list then holds; sh.total_k is the row's mass where k <= 0.
   __device__ bool few(int k, float top_p) {
-    if (threadIdx.x == 0) sh.listed[0] = sh.listed[1] = sh.listed[2] = 0, sh.bin_k = -1;
     histogram(true, k <= 0);
-    if (q.rank == 0) {
-      const uint64_t count = sum_bins(mem.row_counts, kBins, sh);
+    if (q.rank == 0 && threadIdx.x < 32) {
+      uint64_t before = 0, total = 0;
+      int bin_k = -1, border;
+      uint64_t above;
       if (k > 0) {
-        if (threadIdx.x == 0) sh.border = kBins - 1, sh.above = static_cast<int>(count);
-        __syncthreads();
-        if (static_cast<uint64_t>(k) < count)
-          find_bin(mem.row_counts, static_cast<uint64_t>(k), sh, [&](int b, uint64_t before) {
-            sh.border = sh.bin_k = b;
-            sh.above = static_cast<int>(before) + static_cast<int>(mem.row_counts[b]);
-            sh.need = static_cast<uint64_t>(k) - before;
-          });
+        bin_k = find_bin(mem.row_counts, static_cast<uint64_t>(k), &before);
+        border = bin_k < 0 ? kBins - 1 : bin_k;
+        above = bin_k < 0 ? before : before + mem.row_counts[bin_k];
       } else {
-        const uint64_t total = sum_bins(mem.row_masses, kBins, sh);
-        find_bin(mem.row_masses, needed_mass(top_p, total), sh, [&](int b, uint64_t) { sh.border = b; });
-        __syncthreads();
-        const uint64_t above = sum_bins(mem.row_counts, sh.border + 1, sh);
-        if (threadIdx.x == 0) sh.above = static_cast<int>(above), sh.total_k = total;
+        total = sum_bins(mem.row_masses, kBins);
+        uint64_t ahead;
+        border = find_bin(mem.row_masses, needed_mass(top_p, total), &ahead);
+        above = sum_bins(mem.row_counts, border + 1);
+      }
+      if (threadIdx.x == 0) {
+        sh.bin_k = bin_k, sh.border = border, sh.above = static_cast<int>(above);
+        sh.need = static_cast<uint64_t>(k) - before;  // of bin_k
+        sh.total_k = total;
       }
     }
     row_sync(q);
@@ -617,8 +726,10 @@ struct Border {
     if (k > 0) {
       histogram(false, true);
       if (lead) {
-        const uint64_t total = sum_bins(mem.row_masses, kBins, sh);
-        if (tid == 0) sh.total_k = total;
+        if (tid < 32) {
+          const uint64_t total = sum_bins(mem.row_masses, kBins);
+          if (tid == 0) sh.total_k = total;
+        }
         __syncthreads();
       }
       if (bin_k >= 0) {
@@ -652,12 +763,12 @@ struct Border {
     if (!(top_p < 1.f)) return floor;
     if (lead) {
       __syncthreads();
-      const uint64_t need = needed_mass(top_p, sh.total_k);
-      find_bin(mem.row_masses, need, sh, [&](int b, uint64_t before) {
-        sh.bin_p = b;
-        sh.before = before;
-      });
-      if (tid == 0) sh.need = need;
+      if (tid < 32) {
+        const uint64_t need = needed_mass(top_p, sh.total_k);
+        uint64_t before;
+        const int b = find_bin(mem.row_masses, need, &before);
+        if (tid == 0) sh.bin_p = b, sh.before = before, sh.need = need;
+      }
     }
     row_sync(q);
     const int bin_p = *at_rank(&sh.bin_p, q, 0);
@@ -689,11 +800,60 @@ struct Border {
   }
 };
 
+// The places of the block's columns that may weigh anything, in column order, and how many they are;
+// -1 where they are more than half the segment. A row under a grammar mask has few, which the passes
+// that follow then go through without the gaps.
+__device__ __forceinline__ int compact(const Part& q, const float* x, const Weights& weight, int segment,
+                                       uint16_t* places, ChooseShared& sh) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, spans = segment / kSpan;
+  for (int s = warp; s < spans; s += warps) {
+    const float4 v = reinterpret_cast<const float4*>(x + s * kSpan)[lane];
+    const int count = weight.maybe(v.x) + weight.maybe(v.y) + weight.maybe(v.z) + weight.maybe(v.w);
+    const int all = __reduce_add_sync(~0u, count);
+    if (lane == 0) sh.spans[s] = all;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    const int per = (spans + 31) / 32, lo = min(lane * per, spans), hi = min(lo + per, spans);
+    int sum = 0;
+    for (int i = lo; i < hi; ++i) sum += sh.spans[i];
+    int ahead = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(~0u, ahead, o);
+      if (lane >= o) ahead += u;
+    }
+    if (lane == 31) sh.spans[spans] = ahead;
+    ahead -= sum;
+    for (int i = lo; i < hi; ++i) {
+      const int here = sh.spans[i];
+      sh.spans[i] = ahead;
+      ahead += here;
+    }
+  }
+  __syncthreads();
+  const int left = sh.spans[spans];
+  if (left > segment / 2) return -1;
+  const unsigned below = (1u << lane) - 1;
+  for (int s = warp; s < spans; s += warps) {
+    const float4 v = reinterpret_cast<const float4*>(x + s * kSpan)[lane];
+    const bool in[4] = {weight.maybe(v.x), weight.maybe(v.y), weight.maybe(v.z), weight.maybe(v.w)};
+    int at = sh.spans[s];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) at += __popc(__ballot_sync(~0u, in[j]) & below);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (in[j]) places[at++] = static_cast<uint16_t>(s * kSpan + 4 * lane + j);
+  }
+  __syncthreads();
+  return left;
+}
+
 // Cuts off and draws from the n <= 32 G elements of a list, by one warp; `total` is the row's mass
 // where k <= 0, and `kept` shared memory for 32 G weights.
 template <int G>
 __device__ __forceinline__ Choice draw_few(const uint64_t* list, int n, int k, float top_p, uint64_t total,
-                                           const float* uniform, const Weights& weight, uint64_t* kept) {
+                                           const float* uniform, const TableWeights& weight, uint64_t* kept) {
   const int lane = threadIdx.x & 31;
   uint64_t e[G], w[G];
 #pragma unroll
@@ -749,27 +909,26 @@ __device__ __forceinline__ Choice draw_few(const uint64_t* list, int n, int k, f
                 static_cast<float>(static_cast<double>(__shfl_sync(~0u, drawn, owner)) / static_cast<double>(total))};
 }
 
-template <class T, int NQ, bool QUADS>
-__global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(NQ)) choose_wide_kernel(ChooseParams p, int blocks, int segment) {
+template <class T, bool QUADS>
+__global__ void __launch_bounds__(kMaxThreads) choose_wide_kernel(ChooseParams p, int blocks, int segment) {
   extern __shared__ __align__(16) unsigned char dynamic[];
   __shared__ ChooseShared sh;
+  if (threadIdx.x < 32) sh.powers[threadIdx.x] = exp2(threadIdx.x / 32.0);
+  if (threadIdx.x < 4) sh.listed[threadIdx.x] = 0;
   grid_dep_wait();
   grid_dep_launch();
   const Part q = my_part(blocks, segment, p.in.width);
-  const ChooseMemory mem(dynamic, segment, blocks);
+  ChooseMemory mem(dynamic, segment, blocks);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5, row = q.row;
   const float t = p.in.temperature ? p.in.temperature[row] : 1.f;
-  uint32_t best;
-  int first = -1;
-  {
-    float x[NQ][4];
-    load_part<T, NQ, QUADS>(p.in, q, mem.x, x);
-    best = row_best(q, x, sh.best);
-    if (best && best != ~0u && (t <= 0.f || !p.uniform)) first = row_first<NQ, QUADS>(q, x, key_value(best), sh.first);
-#pragma unroll
-    for (int k = 0; k < NQ; ++k)
-      if (span_base(k) < segment) store_span<QUADS>(mem.x, span_base(k), segment, x[k]);
-  }
+  const int k = p.top_k ? p.top_k[row] : 0;
+  const float top_p = p.top_p ? p.top_p[row] : 1.f;
+  const float uniform = p.uniform ? p.uniform[row] : 0.f;
+  float x[kQuads][4], mine;
+  load_part<T, QUADS>(p.in, q, mem.x, x);
+  const uint32_t best = row_best(q, x, sh.best, mine);
+  const float m = key_value(best);
+  const int first = best && best != ~0u && (t <= 0.f || !p.uniform) ? row_first<QUADS>(q, x, m, sh.first) : -1;
   if (best == 0 || best == ~0u || !(t > 0.f)) {
     if (q.rank == 0 && tid == 0) {
       const bool nan = best == ~0u || t != t;
@@ -778,18 +937,23 @@ __global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(NQ)) choose_wide_ke
     row_sync(q);  // no block leaves while another reads from it
     return;
   }
+  const TableWeights weight(m, t, sh.powers);
+#pragma unroll
+  for (int k = 0; k < kQuads; ++k)
+    if (span_base(k) < segment) store_span<QUADS>(mem.x, span_base(k), segment, x[k]);
+  mem.left = -1;
   __syncthreads();
-  const float m = key_value(best);
-  const Weights weight(m, t);
-  const int k = p.top_k ? p.top_k[row] : 0;
-  const float top_p = p.top_p ? p.top_p[row] : 1.f;
   uint64_t last = 0;
+  // Where every weight is needed first, or again, the row is gone through without its gaps.
+  if (k <= 0) mem.left = compact(q, mem.x, weight, segment, mem.places, sh);
   if (k > 0 || top_p < 1.f) {
     Border border{q, mem, sh, weight, m, kBinsPerUnit / t};
-    if (border.few(k, top_p)) {
+    const bool small = k > 0 && border.few_k(mine, k);
+    if (!small && k > 0) mem.left = compact(q, mem.x, weight, segment, mem.places, sh);
+    if (small || border.few(k, top_p)) {
       if (q.rank == 0 && warp == 0) {
-        const int n = static_cast<int>(sh.listed[0]);
-        const float* u = p.uniform ? p.uniform + row : nullptr;
+        const int n = static_cast<int>(sh.listed[small ? 3 : 0]);
+        const float* u = p.uniform ? &uniform : nullptr;
         Choice c;
         if (n <= 32) c = draw_few<1>(mem.list, n, k, top_p, sh.total_k, u, weight, sh.digits);
         else if (n <= 64) c = draw_few<2>(mem.list, n, k, top_p, sh.total_k, u, weight, sh.digits);
@@ -804,14 +968,16 @@ __global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(NQ)) choose_wide_ke
   }
 
   // Column order: each warp takes a run of the block's columns.
-  const int run = ((q.n + warps - 1) / warps + 31) & ~31;
-  const int lo = min(warp * run, q.n), hi = min(lo + run, q.n);
+  const int columns = mem.left >= 0 ? mem.left : q.n;
+  const int run = ((columns + warps - 1) / warps + 31) & ~31;
+  const int lo = min(warp * run, columns), hi = min(lo + run, columns);
+  auto place = [&](int u) { return mem.left >= 0 ? static_cast<int>(mem.places[u]) : u; };
   auto kept = [&](int i) -> uint64_t {
     const float v = mem.x[i];
     return weight.maybe(v) && element(v, q.c0 + i) >= last ? weight(v) : 0;
   };
   uint64_t mass = 0;
-  for (int i = lo + lane; i < hi; i += 32) mass += kept(i);
+  for (int u = lo + lane; u < hi; u += 32) mass += kept(place(u));
   mass = warp_sum_u64(mass);
   if (lane == 0) sh.scan[warp] = mass;
   __syncthreads();
@@ -835,16 +1001,17 @@ __global__ void __launch_bounds__(kMaxThreads, blocks_per_sm(NQ)) choose_wide_ke
   if (!p.uniform) {
     if (q.rank == 0 && tid == 0) write_choice(p, row, Choice{first, static_cast<float>(kWeightOne / static_cast<double>(total))});
   } else {
-    const uint64_t unit = drawn_unit(p.uniform[row], total);
+    const uint64_t unit = drawn_unit(uniform, total);
     ahead += sh.scan[warp];
     const uint64_t end = ahead + sh.scan[warp + 1] - sh.scan[warp];
     if (unit >= ahead && unit < end) {
-      for (int i0 = lo; i0 < hi; i0 += 32) {
-        const uint64_t w = i0 + lane < hi ? kept(i0 + lane) : 0;
+      for (int u0 = lo; u0 < hi; u0 += 32) {
+        const int i = u0 + lane < hi ? place(u0 + lane) : 0;
+        const uint64_t w = u0 + lane < hi ? kept(i) : 0;
         const uint64_t before = ahead + warp_exclusive_u64(w, lane);
         const bool here = w && unit >= before && unit < before + w;
         if (here)
-          write_choice(p, row, Choice{q.c0 + i0 + lane, static_cast<float>(static_cast<double>(w) / static_cast<double>(total))});
+          write_choice(p, row, Choice{q.c0 + i, static_cast<float>(static_cast<double>(w) / static_cast<double>(total))});
         ahead = __shfl_sync(~0u, before + w, 31);
         if (__any_sync(~0u, here)) break;
       }
@@ -871,26 +1038,16 @@ Shape wide_shape(const LogitParams& p) {
   Shape s;
   s.blocks = blocks;
   s.segment = ((width + blocks - 1) / blocks + kSpan - 1) / kSpan * kSpan;
-  const int per_thread = 4 * (s.segment > kMaxThreads * 4 * kQuadsNarrow ? kQuadsWide : kQuadsNarrow);
-  s.threads = (s.segment + 32 * per_thread - 1) / (32 * per_thread) * 32;
+  s.threads = (s.segment + kQuads * kSpan - 1) / (kQuads * kSpan) * 32;
   if (s.threads < 128) s.threads = 128;
   return s;
 }
 
-// f(type, quads per thread, whether they are read at once) for the instantiations. Rows of quads: each
-// row of logits and of the outputs starts on a boundary of four elements.
-template <int N>
-using Int = std::integral_constant<int, N>;
-
+// f(type, whether four columns are read at once) for the instantiations. They are where each row of
+// logits and of the outputs starts on a boundary of four elements.
 template <class F>
-cudaError_t with_wide(const LogitParams& p, const Shape& shape, bool quads, F&& f) {
-  return with_type(p.type, [&](auto v) {
-    auto with_quads = [&](auto q) {
-      if (shape.segment > kMaxThreads * 4 * kQuadsNarrow) return f(v, Int<kQuadsWide>(), q);
-      return f(v, Int<kQuadsNarrow>(), q);
-    };
-    return quads ? with_quads(std::true_type()) : with_quads(std::false_type());
-  });
+cudaError_t with_wide(const LogitParams& p, bool quads, F&& f) {
+  return with_type(p.type, [&](auto v) { return quads ? f(v, std::true_type()) : f(v, std::false_type()); });
 }
 
 bool quad_rows(const void* base, int64_t stride, int size) {
@@ -926,8 +1083,8 @@ cudaError_t launch_adjust_wide(const AdjustParams& p, cudaStream_t s) {
   const bool quads = quad_rows(p.in) && (!p.out || quad_rows(p.out, p.out_stride, p.in.type == LogitType::kF32 ? 4 : 2)) &&
                      (!p.priors || quad_rows(p.priors, p.priors_stride, 4));
   const size_t smem = p.in.rules.history || p.in.rules.columns ? shape.segment * sizeof(float) : 0;
-  return with_wide(p.in, shape, quads, [&](auto v, auto n, auto q) {
-    return launch_rows(adjust_wide_kernel<decltype(v), n.value, q.value>, p.in.rows, shape, smem, s, p, shape.blocks,
+  return with_wide(p.in, quads, [&](auto v, auto q) {
+    return launch_rows(adjust_wide_kernel<decltype(v), q.value>, p.in.rows, shape, smem, s, p, shape.blocks,
                        shape.segment);
   });
 }
@@ -935,29 +1092,27 @@ cudaError_t launch_adjust_wide(const AdjustParams& p, cudaStream_t s) {
 cudaError_t launch_choose_wide(const ChooseParams& p, cudaStream_t s) {
   const Shape shape = wide_shape(p.in);
   const size_t smem = ChooseMemory::bytes(shape.segment, shape.blocks, p.top_k || p.top_p);
-  return with_wide(p.in, shape, quad_rows(p.in), [&](auto v, auto n, auto q) {
-    return launch_rows(choose_wide_kernel<decltype(v), n.value, q.value>, p.in.rows, shape, smem, s, p, shape.blocks,
+  return with_wide(p.in, quad_rows(p.in), [&](auto v, auto q) {
+    return launch_rows(choose_wide_kernel<decltype(v), q.value>, p.in.rows, shape, smem, s, p, shape.blocks,
                        shape.segment);
   });
 }
 
 cudaError_t prepare_policy_wide() {
   for (LogitType t : {LogitType::kF32, LogitType::kF16, LogitType::kBf16})
-    for (int segment : {kMaxThreads * 4 * kQuadsNarrow, kMaxSegment})
-      for (bool quads : {false, true}) {
-        LogitParams in{};
-        in.type = t;
-        const cudaError_t e = with_wide(in, Shape{1, segment, 0}, quads, [&](auto v, auto n, auto q) {
-          const cudaError_t r =
-              cudaFuncSetAttribute(adjust_wide_kernel<decltype(v), n.value, q.value>,
-                                   cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(segment * sizeof(float)));
-          if (r != cudaSuccess) return r;
-          return cudaFuncSetAttribute(choose_wide_kernel<decltype(v), n.value, q.value>,
-                                      cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      static_cast<int>(ChooseMemory::bytes(segment, kMaxBlocks, true)));
-        });
-        if (e != cudaSuccess) return e;
-      }
+    for (bool quads : {false, true}) {
+      LogitParams in{};
+      in.type = t;
+      const cudaError_t e = with_wide(in, quads, [&](auto v, auto q) {
+        const cudaError_t r = cudaFuncSetAttribute(adjust_wide_kernel<decltype(v), q.value>,
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   static_cast<int>(kMaxSegment * sizeof(float)));
+        if (r != cudaSuccess) return r;
+        return cudaFuncSetAttribute(choose_wide_kernel<decltype(v), q.value>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    static_cast<int>(ChooseMemory::bytes(kMaxSegment, kMaxBlocks, true)));
+      });
+      if (e != cudaSuccess) return e;
+    }
   return cudaSuccess;
 }
 
