@@ -392,7 +392,7 @@ __device__ __forceinline__ Choice draw_narrow(const ChooseParams& p, int row, in
     }
     total = warp_sum_u64(mine);
   }
-  if (!p.uniform) return Choice{-1, static_cast<float>(kWeightOne / static_cast<double>(total))};  // the largest's
+  if (!p.uniform) return Choice{-1, share_of(static_cast<uint64_t>(kWeightOne), total)};  // the largest's
   const uint64_t unit = drawn_unit(p.uniform[row], total);
   uint64_t mine = 0;
 #pragma unroll
@@ -408,7 +408,7 @@ __device__ __forceinline__ Choice draw_narrow(const ChooseParams& p, int row, in
   const int owner = __ffs(__ballot_sync(~0u, place >= 0)) - 1;
   place = __shfl_sync(~0u, place, owner);
   w = __shfl_sync(~0u, w, owner);
-  return Choice{sh.column[place], static_cast<float>(static_cast<double>(w) / static_cast<double>(total))};
+  return Choice{sh.column[place], share_of(w, total)};
 }
 
 template <class T, int K, bool SLOTS>

@@ -59,21 +59,60 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 // and a row in a million would fall on another column than by the definition.
 constexpr double kWeightOne = 1099511627776.0;  // 2^40; a row's 2^18 columns sum to at most 2^58
 
+// 2^(i / 32).
+static __device__ const double kPowers[32] = {
+    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
+    0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0,
+    0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
+    0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0, 0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0,
+    0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
+    0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0,
+};
+
+// 1 / v to a few units of the last place: the f32 reciprocal and two steps of Newton's iteration, which
+// take a fraction of a division's time. v lies between 1e-30 and 1e30.
+__device__ __forceinline__ double reciprocal(double v) {
+  double r = 1.f / static_cast<float>(v);
+  r = r * (2.0 - v * r);
+  return r * (2.0 - v * r);
+}
+
+// The weight of a logit: with 32 z log2(e) = n + f for z = (x - m) / t, n whole and |f| <= 1/2, exp(z) is
+// 2^(n / 32) exp(f ln 2 / 32), the first factor 2^(n >> 5) times one of 32 values, the second the first
+// six terms of its series, the next one below 3e-15. About 15 operations in f64 where exp() takes
+// several times as many.
 struct Weights {
-  double m, inv_t;
-  bool infinite;  // the largest logit is +inf: the columns that hold it share the row
+  double m, steps;  // the largest logit; 32 log2(e) / t
+  bool infinite;    // the largest logit is +inf: the columns that hold it share the row
   float m32, inv_t32;
-  __device__ __forceinline__ Weights(float max, float t)
-      : m(max), inv_t(1.0 / static_cast<double>(t)), infinite(max == INFINITY), m32(max), inv_t32(1.f / t) {}
+  __device__ __forceinline__ Weights(float max, float t) : m(max), infinite(max == INFINITY), m32(max), inv_t32(1.f / t) {
+    steps = 46.166241308446828 * (t > 1e-30f && t < 1e30f ? reciprocal(t) : 1.0 / static_cast<double>(t));
+  }
   // False only for logits that weigh 0: below -41 ln 2 = -28.42 the weight rounds to 0, and three
   // roundings in f32 move -28.5 by less than 1e-5.
   __device__ __forceinline__ bool maybe(float x) const { return !((x - m32) * inv_t32 < -28.5f) && x > -INFINITY; }
   __device__ __forceinline__ uint64_t operator()(float x) const {
     if (!maybe(x)) return 0;
     if (infinite) return x == INFINITY ? static_cast<uint64_t>(kWeightOne) : 0;
-    return static_cast<uint64_t>(__double2ll_rn(exp((static_cast<double>(x) - m) * inv_t) * kWeightOne));
+    constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
+    const double y = (static_cast<double>(x) - m) * steps;
+    const double rounded = y + kRound;
+    const int n = __double2loint(rounded);
+    const double u = (y - (rounded - kRound)) * 0.021660849392498290;  // ln 2 / 32
+    const double series = 1.0 + u * (1.0 + u * (0.5 + u * (1.0 / 6 + u * (1.0 / 24 + u * (1.0 / 120)))));
+    const double power = __ldg(kPowers + (n & 31));  // times 2^(40 + (n >> 5)), through its exponent
+    const double scaled = __hiloint2double(__double2hiint(power) + ((40 + (n >> 5)) << 20), __double2loint(power));
+    constexpr double kWhole = 4503599627370496.0;  // 2^52: the sum's low bits are the rounded product
+    return static_cast<uint64_t>(__double_as_longlong(scaled * series + kWhole)) & ((1ull << 52) - 1);
   }
 };
+
+// w / total, rounded once to f32 (up to a part in 2^40 of a step).
+__device__ __forceinline__ float share_of(uint64_t w, uint64_t total) {
+  return static_cast<float>(static_cast<double>(w) * reciprocal(static_cast<double>(total)));
+}
 
 // The whole number of weight units that a share of the mass needs.
 __device__ __forceinline__ uint64_t needed_mass(float top_p, uint64_t mass) {

@@ -25,6 +25,7 @@ constexpr int kMaxWarps = kMaxThreads / 32;
 constexpr int kMaxBlocks = 8;  // of a cluster; what every device schedules
 constexpr int kMaxSegment = kPolicyMaxWidth / kMaxBlocks;
 constexpr int kQuads = 8;  // columns a thread holds, over four
+static_assert(4 * kQuads <= 32, "a bit for each column of a thread");
 constexpr int kListed = 512;  // entries of a bias list held at a time
 constexpr int kSpan = 128;  // columns that a warp takes at a time, four to a lane
 
@@ -283,12 +284,11 @@ __device__ __forceinline__ void load_part(const LogitParams& p, const Part& q, f
 // left holds NaN.
 __device__ __forceinline__ uint32_t row_best(const Part& q, const float (&x)[kQuads][4], Exchange<uint32_t>& ex, float& m) {
   m = -INFINITY;  // of this thread
-  bool nan = false;
 #pragma unroll
   for (int k = 0; k < kQuads; ++k)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) m = fmaxf(m, x[k][j]), nan |= x[k][j] != x[k][j];
-  const uint32_t key = nan ? ~0u : m == -INFINITY ? 0u : order_key(m);
+    for (int j = 0; j < 4; ++j) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(x[k][j]));
+  const uint32_t key = m != m ? ~0u : m == -INFINITY ? 0u : order_key(m);
   return row_reduce(q, key, [](uint32_t a, uint32_t b) { return a > b ? a : b; }, ex);
 }
 
@@ -333,37 +333,40 @@ __global__ void __launch_bounds__(kMaxThreads) adjust_wide_kernel(AdjustParams p
   float mine;
   const uint32_t best = row_best(q, x, ex_best, mine);
   const float m = key_value(best);
-  float sum = 0.f;
-  if (best != ~0u && (t <= 0.f || m == INFINITY)) {
-    // the largest logit's lowest column, or the columns at +inf
-    const int first = t <= 0.f && best ? row_first<QUADS>(q, x, m, ex_first) : -1;
+  float sum = 0.f, inv;
+  auto total = [&]() { return row_reduce(q, sum, [](float a, float b) { return a + b; }, ex_sum); };
+  if (best && best != ~0u && t > 0.f && m != INFINITY) {
+    // exp((x - m) / t). The scale is finite and not 0, so that 0 stays 0 and -inf stays -inf under it.
+    const float scale = fmaxf(fminf(1.44269504088896341f / t, 3.4e38f), 1.5e-45f);
 #pragma unroll
     for (int k = 0; k < kQuads; ++k)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        // (a thread's columns behind the segment, all -inf, are numbered like the next block's)
-        x[k][j] = t <= 0.f ? x[k][j] == m && q.c0 + span_base(k) + span_column<QUADS>(j) == first : t != t && x[k][j] > -INFINITY ? NAN : x[k][j] == m;
+        x[k][j] = power_of_two((x[k][j] - m) * scale);
         sum += x[k][j];
       }
+    inv = 1.f / total();
   } else {
-    // exp((x - m) / t); NaN, in the row or as t, runs through
-    const float top = best ? m : 0.f;
-    const float scale = t != t ? t : fminf(1.44269504088896341f / t, 3.4e38f);  // finite: 0 * scale is 0
+    // Nothing left: 0. A NaN, in the row or as t: NaN wherever something is left. Else the largest
+    // logit's lowest column, or the columns at +inf.
+    const bool nan = best == ~0u || t != t;
+    const int first = !nan && best && t <= 0.f ? row_first<QUADS>(q, x, m, ex_first) : -1;
 #pragma unroll
     for (int k = 0; k < kQuads; ++k)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        x[k][j] = x[k][j] == -INFINITY ? 0.f : power_of_two((x[k][j] - top) * scale);
-        sum += x[k][j];
+        const bool there = x[k][j] == m && (t > 0.f || q.c0 + span_base(k) + span_column<QUADS>(j) == first);
+        x[k][j] = x[k][j] == -INFINITY ? 0.f : nan ? NAN : there ? 1.f : 0.f;
+        if (!nan) sum += x[k][j];
       }
+    sum = total();
+    inv = sum == 0.f ? 1.f : 1.f / sum;
   }
-  sum = row_reduce(q, sum, [](float a, float b) { return a + b; }, ex_sum);
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   float* priors = p.priors + q.row * p.priors_stride + q.c0;
 #pragma unroll
   for (int k = 0; k < kQuads; ++k) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[k][j] = x[k][j] == 0.f ? 0.f : x[k][j] * inv;  // a masked column stays 0 beside a NaN
+    for (int j = 0; j < 4; ++j) x[k][j] *= inv;
     store_span<QUADS>(priors, span_base(k), q.n, x[k]);
   }
   if (q.blocks > 1) cg::this_cluster().sync();  // no block leaves while another reads from it
@@ -385,7 +388,6 @@ constexpr int kFew = 256;
 __host__ __device__ constexpr int list_capacity(int segment) { return segment <= 8192 ? 1024 : 4096; }
 
 struct ChooseShared {
-  double powers[32];  // 2^(i / 32)
   int spans[kMaxSegment / kSpan + 1];  // columns that may weigh anything before each span
   Exchange<uint32_t> best;
   Exchange<int> first;
@@ -431,31 +433,6 @@ struct ChooseMemory {
   }
 };
 
-// Weights (policy_rows.cuh) by a table: with 32 z log2(e) = n + f, n whole and |f| <= 1/2, exp(z) is
-// 2^(n / 32) exp(f ln 2 / 32), the first factor 2^(n >> 5) times one of 32 values, the second the first
-// six terms of its series, the next one below 3e-15. About 15 operations in f64 where exp() takes
-// several times as many: a wide row's f64 pipe is what these kernels run out of first.
-struct TableWeights : Weights {
-  double steps;  // 32 log2(e) / t
-  const double* table;
-  __device__ __forceinline__ TableWeights(float max, float t, const double* powers)
-      : Weights(max, t), steps(46.166241308446828 * inv_t), table(powers) {}
-  __device__ __forceinline__ uint64_t operator()(float x) const {
-    if (!maybe(x)) return 0;
-    if (infinite) return x == INFINITY ? static_cast<uint64_t>(kWeightOne) : 0;
-    constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
-    const double y = (static_cast<double>(x) - m) * steps;
-    const double rounded = y + kRound;
-    const int n = __double2loint(rounded);
-    const double u = (y - (rounded - kRound)) * 0.021660849392498290;  // ln 2 / 32
-    const double series = 1.0 + u * (1.0 + u * (0.5 + u * (1.0 / 6 + u * (1.0 / 24 + u * (1.0 / 120)))));
-    const double power = table[n & 31];  // times 2^(40 + (n >> 5)), through its exponent
-    const double scaled = __hiloint2double(__double2hiint(power) + ((40 + (n >> 5)) << 20), __double2loint(power));
-    constexpr double kWhole = 4503599627370496.0;  // 2^52: the sum's low bits are the rounded product
-    return static_cast<uint64_t>(__double_as_longlong(scaled * series + kWhole)) & ((1ull << 52) - 1);
-  }
-};
-
 __device__ __forceinline__ uint64_t element(float x, int column) {
   return static_cast<uint64_t>(order_key(x)) << 32 | ~static_cast<uint32_t>(column);
 }
@@ -489,34 +466,51 @@ __device__ __forceinline__ uint64_t block_exclusive_u64(uint64_t v, ChooseShared
   return before + in - v;
 }
 
-// Sum of bins [0, end), by one warp.
+// Sums over a row's histogram, by one warp: of groups of 32 bins first, all of them at once.
 template <class V>
-__device__ __forceinline__ uint64_t sum_bins(const V* values, int end) {
-  uint64_t sum = 0;
-  for (int b = threadIdx.x & 31; b < end; b += 32) sum += values[b];
-  return warp_sum_u64(sum);
-}
+struct BinSums {
+  static constexpr int kGroups = kBins / 32;
+  const V* values;
+  V sums[kGroups];
 
-// The bin at which the sums of `values` from bin 0 on reach `need`, and the sum of the bins before it,
-// by one warp; -1, and the sum of all, where they never do.
-template <class V>
-__device__ __forceinline__ int find_bin(const V* values, uint64_t need, uint64_t* before) {
-  const int lane = threadIdx.x & 31;
-  uint64_t ahead = 0;
-  for (int b0 = 0; b0 < kBins; b0 += 32) {
-    const uint64_t v = values[b0 + lane];
-    const uint64_t mine = ahead + warp_exclusive_u64(v, lane);
-    const unsigned reached = __ballot_sync(~0u, mine + v >= need);
-    if (reached) {
-      const int first = __ffs(reached) - 1;
-      *before = __shfl_sync(~0u, mine, first);
-      return b0 + first;
+  __device__ __forceinline__ explicit BinSums(const V* bins) : values(bins) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) sums[g] = values[32 * g + lane];
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      if constexpr (sizeof(V) == 4) sums[g] = __reduce_add_sync(~0u, sums[g]);
+      else sums[g] = warp_sum_u64(sums[g]);
     }
-    ahead = __shfl_sync(~0u, mine + v, 31);
   }
-  *before = ahead;
-  return -1;
-}
+  __device__ __forceinline__ uint64_t total() const {
+    uint64_t sum = 0;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) sum += sums[g];
+    return sum;
+  }
+  // The bin at which the sums from bin 0 on reach `need`, and the sum of the bins before it; -1, and the
+  // sum of all, where they never do.
+  __device__ __forceinline__ int reach(uint64_t need, uint64_t* before) const {
+    uint64_t ahead = 0;
+    int group = -1;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      if (group < 0) {
+        if (ahead + sums[g] >= need) group = g;
+        else ahead += sums[g];
+      }
+    }
+    *before = ahead;
+    if (group < 0) return -1;
+    const int lane = threadIdx.x & 31;
+    const uint64_t here = values[32 * group + lane];
+    const uint64_t mine = ahead + warp_exclusive_u64(here, lane);
+    const int first = __ffs(__ballot_sync(~0u, mine + here >= need)) - 1;
+    *before = __shfl_sync(~0u, mine, first);
+    return 32 * group + first;
+  }
+};
 
 // Sorts list[0, n), largest first, by one block. The list holds a power of two of at least n.
 __device__ __forceinline__ void sort_list(uint64_t* list, int n) {
@@ -536,11 +530,50 @@ __device__ __forceinline__ void sort_list(uint64_t* list, int n) {
   __syncthreads();
 }
 
+// The element at rank `need` - 1 of list[0, n), counted from the largest, or the one at which the
+// weights reach `need`, into *found, by one block.
+template <class W>
+__device__ __forceinline__ void reach_in_list(uint64_t* list, int n, bool masses, uint64_t need, const W& weight,
+                                              ChooseShared& sh, uint64_t* found) {
+  const int threads = blockDim.x;
+  if (n > kFew) {
+    sort_list(list, n);
+    const int per = (n + threads - 1) / threads;
+    const int lo = min(static_cast<int>(threadIdx.x) * per, n), hi = min(lo + per, n);
+    auto of = [&](int i) { return masses ? weight(key_value(static_cast<uint32_t>(list[i] >> 32))) : 1; };
+    uint64_t mine = 0, total;
+    for (int i = lo; i < hi; ++i) mine += of(i);
+    uint64_t ahead = block_exclusive_u64(mine, sh, &total);
+    if (ahead < need && need <= ahead + mine)
+      for (int i = lo; i < hi; ++i) {
+        ahead += of(i);
+        if (ahead >= need) {
+          *found = list[i];
+          break;
+        }
+      }
+  } else {
+    // A short list is not sorted: every element adds up what lies ahead of it.
+    for (int i = threadIdx.x; i < n; i += threads)
+      sh.digits[i] = masses ? weight(key_value(static_cast<uint32_t>(list[i] >> 32))) : 1;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += threads) {
+      const uint64_t e = list[i];
+      uint64_t ahead = 0;
+#pragma unroll 4
+      for (int j = 0; j < n; ++j)
+        if (list[j] > e) ahead += sh.digits[j];
+      if (ahead < need && need <= ahead + sh.digits[i]) *found = e;
+    }
+  }
+  __syncthreads();
+}
+
 struct Border {
   const Part& q;
   const ChooseMemory& mem;
   ChooseShared& sh;
-  const TableWeights& weight;
+  const Weights& weight;
   float m, per_bin;
 
   __device__ __forceinline__ int bin(float x) const {
@@ -676,7 +709,7 @@ struct Border {
     add_up(true, false);
     if (q.rank == 0 && threadIdx.x < 32) {
       uint64_t before;
-      const int b = find_bin(mem.row_counts, static_cast<uint64_t>(k), &before);
+      const int b = BinSums<uint32_t>(mem.row_counts).reach(static_cast<uint64_t>(k), &before);
       if (threadIdx.x == 0) sh.border = b < 0 ? kBins - 1 : b;
     }
     row_sync(q);
@@ -692,21 +725,25 @@ struct Border {
     if (q.rank == 0 && threadIdx.x < 32) {
       uint64_t before = 0, total = 0;
       int bin_k = -1, border;
-      uint64_t above;
+      uint64_t above, ahead = 0, need = 0;
       if (k > 0) {
-        bin_k = find_bin(mem.row_counts, static_cast<uint64_t>(k), &before);
+        bin_k = BinSums<uint32_t>(mem.row_counts).reach(static_cast<uint64_t>(k), &before);
         border = bin_k < 0 ? kBins - 1 : bin_k;
         above = bin_k < 0 ? before : before + mem.row_counts[bin_k];
       } else {
-        total = sum_bins(mem.row_masses, kBins);
-        uint64_t ahead;
-        border = find_bin(mem.row_masses, needed_mass(top_p, total), &ahead);
-        above = sum_bins(mem.row_counts, border + 1);
+        const BinSums<uint64_t> masses(mem.row_masses);
+        total = masses.total();
+        need = needed_mass(top_p, total);
+        border = masses.reach(need, &ahead);
+        above = 0;
+        for (int b = threadIdx.x; b <= border; b += 32) above += mem.row_counts[b];
+        above = warp_sum_u64(above);
       }
       if (threadIdx.x == 0) {
         sh.bin_k = bin_k, sh.border = border, sh.above = static_cast<int>(above);
-        sh.need = static_cast<uint64_t>(k) - before;  // of bin_k
-        sh.total_k = total;
+        // of bin_k, or of bin_p
+        sh.need = k > 0 ? static_cast<uint64_t>(k) - before : need;
+        sh.bin_p = border, sh.before = ahead, sh.total_k = total;
       }
     }
     row_sync(q);
@@ -721,13 +758,13 @@ struct Border {
     const int tid = threadIdx.x, threads = blockDim.x;
     const bool lead = q.rank == 0;
     uint64_t floor = 0;
-    bool listed = false;  // the first block's list holds bin_k, sorted
+    bool listed = false;  // the first block's list holds bin_k
     const int bin_k = *at_rank(&sh.bin_k, q, 0);
     if (k > 0) {
       histogram(false, true);
       if (lead) {
         if (tid < 32) {
-          const uint64_t total = sum_bins(mem.row_masses, kBins);
+          const uint64_t total = BinSums<uint64_t>(mem.row_masses).total();
           if (tid == 0) sh.total_k = total;
         }
         __syncthreads();
@@ -738,13 +775,14 @@ struct Border {
         listed = *at_rank(&sh.listed[1], q, 0) <= mem.room;
         if (listed) {
           if (lead) {
-            const int n = static_cast<int>(sh.listed[1]), keep = static_cast<int>(sh.need);
-            sort_list(mem.list, n);
+            const int n = static_cast<int>(sh.listed[1]);
+            reach_in_list(mem.list, n, false, sh.need, weight, sh, &sh.threshold);
             uint64_t mass = 0, total;
             for (int b = tid; b < bin_k; b += threads) mass += mem.row_masses[b];
-            for (int i = tid; i < keep; i += threads) mass += weight(key_value(static_cast<uint32_t>(mem.list[i] >> 32)));
+            for (int i = tid; i < n; i += threads)
+              if (mem.list[i] >= sh.threshold) mass += weight(key_value(static_cast<uint32_t>(mem.list[i] >> 32)));
             block_exclusive_u64(mass, sh, &total);
-            if (tid == 0) sh.threshold = mem.list[keep - 1], sh.total_k = total;
+            if (tid == 0) sh.total_k = total;
           }
           row_sync(q);
           floor = *at_rank(&sh.threshold, q, 0);
@@ -761,39 +799,28 @@ struct Border {
       }
     }
     if (!(top_p < 1.f)) return floor;
-    if (lead) {
-      __syncthreads();
-      if (tid < 32) {
-        const uint64_t need = needed_mass(top_p, sh.total_k);
-        uint64_t before;
-        const int b = find_bin(mem.row_masses, need, &before);
-        if (tid == 0) sh.bin_p = b, sh.before = before, sh.need = need;
+    if (k > 0) {
+      if (lead) {
+        __syncthreads();
+        if (tid < 32) {
+          const uint64_t need = needed_mass(top_p, sh.total_k);
+          uint64_t before;
+          const int b = BinSums<uint64_t>(mem.row_masses).reach(need, &before);
+          if (tid == 0) sh.bin_p = b, sh.before = before, sh.need = need;
+        }
       }
+      row_sync(q);
     }
-    row_sync(q);
     const int bin_p = *at_rank(&sh.bin_p, q, 0);
     const bool again = bin_p != bin_k || !listed;
     if (again) {
       gather(bin_p, bin_p, 2);
       row_sync(q);
       if (*at_rank(&sh.listed[2], q, 0) > mem.room) return by_digits(*at_rank(&sh.need, q, 0), floor, true);
-      if (lead) sort_list(mem.list, static_cast<int>(sh.listed[2]));
     }
     if (lead) {
       __syncthreads();
-      const int n = static_cast<int>(sh.listed[again ? 2 : 1]);
-      const int per = (n + threads - 1) / threads, lo = min(tid * per, n), hi = min(lo + per, n);
-      uint64_t mine = 0, total;
-      for (int i = lo; i < hi; ++i) mine += weight(key_value(static_cast<uint32_t>(mem.list[i] >> 32)));
-      uint64_t ahead = sh.before + block_exclusive_u64(mine, sh, &total);
-      if (ahead < sh.need && sh.need <= ahead + mine)
-        for (int i = lo; i < hi; ++i) {
-          ahead += weight(key_value(static_cast<uint32_t>(mem.list[i] >> 32)));
-          if (ahead >= sh.need) {
-            sh.threshold = mem.list[i];
-            break;
-          }
-        }
+      reach_in_list(mem.list, static_cast<int>(sh.listed[again ? 2 : 1]), true, sh.need - sh.before, weight, sh, &sh.threshold);
     }
     row_sync(q);
     return *at_rank(&sh.threshold, q, 0);
@@ -852,8 +879,8 @@ __device__ __forceinline__ int compact(const Part& q, const float* x, const Weig
 // Cuts off and draws from the n <= 32 G elements of a list, by one warp; `total` is the row's mass
 // where k <= 0, and `kept` shared memory for 32 G weights.
 template <int G>
-__device__ __forceinline__ Choice draw_few(const uint64_t* list, int n, int k, float top_p, uint64_t total,
-                                           const float* uniform, const TableWeights& weight, uint64_t* kept) {
+__device__ __forceinline__ Choice draw_sorted(const uint64_t* list, int n, int k, float top_p, uint64_t total,
+                                           const float* uniform, const Weights& weight, uint64_t* kept) {
   const int lane = threadIdx.x & 31;
   uint64_t e[G], w[G];
 #pragma unroll
@@ -886,7 +913,7 @@ __device__ __forceinline__ Choice draw_few(const uint64_t* list, int n, int k, f
     e[g] = w[g] ? e[g] << 32 | static_cast<uint32_t>(lane * G + g) : 0;
   }
   total = warp_sum_u64(mine);
-  if (!uniform) return Choice{-1, static_cast<float>(kWeightOne / static_cast<double>(total))};  // the largest's
+  if (!uniform) return Choice{-1, share_of(static_cast<uint64_t>(kWeightOne), total)};  // the largest's
   const uint64_t unit = drawn_unit(*uniform, total);
   warp_sort<G>(e, lane);
   __syncwarp();
@@ -906,14 +933,71 @@ __device__ __forceinline__ Choice draw_few(const uint64_t* list, int n, int k, f
   }
   const int owner = __ffs(__ballot_sync(~0u, column >= 0)) - 1;
   return Choice{__shfl_sync(~0u, column, owner),
-                static_cast<float>(static_cast<double>(__shfl_sync(~0u, drawn, owner)) / static_cast<double>(total))};
+                share_of(__shfl_sync(~0u, drawn, owner), total)};
+}
+
+// Cuts off and draws from the n <= kFew elements of a list, by one block; `total` is the row's mass where
+// k <= 0. Nothing is sorted: each element counts what lies ahead of it, first by logit and then by
+// column, which takes n steps of two short loops on all threads at once.
+__device__ __forceinline__ void draw_few(const ChooseParams& p, int row, const uint64_t* list, int n, int k, float top_p,
+                                         uint64_t total, float uniform, int first, const Weights& weight,
+                                         ChooseShared& sh) {
+  const int tid = threadIdx.x, threads = blockDim.x;
+  if (n <= 64) {
+    // The shortest lists: one warp, without a barrier.
+    if (tid >= 32) return;
+    const float* u = p.uniform ? &uniform : nullptr;
+    Choice c = n <= 32 ? draw_sorted<1>(list, n, k, top_p, total, u, weight, sh.digits)
+                       : draw_sorted<2>(list, n, k, top_p, total, u, weight, sh.digits);
+    if (!u) c.column = first;
+    if (tid == 0) write_choice(p, row, c);
+    return;
+  }
+  uint64_t* w = sh.digits;
+  for (int i = tid; i < n; i += threads) w[i] = weight(key_value(static_cast<uint32_t>(list[i] >> 32)));
+  __syncthreads();
+  uint64_t mass = 0;
+  uint64_t* ahead = sh.digit_sums;
+  for (int i = tid; i < n; i += threads) {
+    const uint64_t e = list[i];
+    uint64_t sum = 0;
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j)
+      if (list[j] > e) ++rank, sum += w[j];
+    const bool in = k <= 0 || rank < k;
+    ahead[i] = in ? sum : ~0ull;
+    if (in) mass += w[i];
+  }
+  if (k > 0) block_exclusive_u64(mass, sh, &total);
+  const uint64_t need = top_p < 1.f ? needed_mass(top_p, total) : ~0ull;
+  mass = 0;
+  __syncthreads();
+  for (int i = tid; i < n; i += threads) {
+    if (ahead[i] >= need) w[i] = 0;
+    mass += w[i];
+  }
+  block_exclusive_u64(mass, sh, &total);
+  if (!p.uniform) {
+    if (tid == 0) write_choice(p, row, Choice{first, share_of(static_cast<uint64_t>(kWeightOne), total)});
+    return;
+  }
+  const uint64_t unit = drawn_unit(uniform, total);
+  for (int i = tid; i < n; i += threads) {
+    const uint32_t place = static_cast<uint32_t>(list[i]);  // ~column
+    uint64_t before = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j)
+      if (static_cast<uint32_t>(list[j]) > place) before += w[j];
+    if (unit >= before && unit < before + w[i])
+      write_choice(p, row, Choice{static_cast<int>(~place), share_of(w[i], total)});
+  }
 }
 
 template <class T, bool QUADS>
 __global__ void __launch_bounds__(kMaxThreads) choose_wide_kernel(ChooseParams p, int blocks, int segment) {
   extern __shared__ __align__(16) unsigned char dynamic[];
   __shared__ ChooseShared sh;
-  if (threadIdx.x < 32) sh.powers[threadIdx.x] = exp2(threadIdx.x / 32.0);
   if (threadIdx.x < 4) sh.listed[threadIdx.x] = 0;
   grid_dep_wait();
   grid_dep_launch();
@@ -937,7 +1021,7 @@ __global__ void __launch_bounds__(kMaxThreads) choose_wide_kernel(ChooseParams p
     row_sync(q);  // no block leaves while another reads from it
     return;
   }
-  const TableWeights weight(m, t, sh.powers);
+  const Weights weight(m, t);
 #pragma unroll
   for (int k = 0; k < kQuads; ++k)
     if (span_base(k) < segment) store_span<QUADS>(mem.x, span_base(k), segment, x[k]);
@@ -951,17 +1035,8 @@ __global__ void __launch_bounds__(kMaxThreads) choose_wide_kernel(ChooseParams p
     const bool small = k > 0 && border.few_k(mine, k);
     if (!small && k > 0) mem.left = compact(q, mem.x, weight, segment, mem.places, sh);
     if (small || border.few(k, top_p)) {
-      if (q.rank == 0 && warp == 0) {
-        const int n = static_cast<int>(sh.listed[small ? 3 : 0]);
-        const float* u = p.uniform ? &uniform : nullptr;
-        Choice c;
-        if (n <= 32) c = draw_few<1>(mem.list, n, k, top_p, sh.total_k, u, weight, sh.digits);
-        else if (n <= 64) c = draw_few<2>(mem.list, n, k, top_p, sh.total_k, u, weight, sh.digits);
-        else if (n <= 128) c = draw_few<4>(mem.list, n, k, top_p, sh.total_k, u, weight, sh.digits);
-        else c = draw_few<8>(mem.list, n, k, top_p, sh.total_k, u, weight, sh.digits);
-        if (!u) c.column = first;
-        if (lane == 0) write_choice(p, row, c);
-      }
+      if (q.rank == 0)
+        draw_few(p, row, mem.list, static_cast<int>(sh.listed[small ? 3 : 0]), k, top_p, sh.total_k, uniform, first, weight, sh);
       return;  // the first block reads its own memory only
     }
     last = border.find(k, top_p);
@@ -999,7 +1074,7 @@ __global__ void __launch_bounds__(kMaxThreads) choose_wide_kernel(ChooseParams p
     total += here;
   }
   if (!p.uniform) {
-    if (q.rank == 0 && tid == 0) write_choice(p, row, Choice{first, static_cast<float>(kWeightOne / static_cast<double>(total))});
+    if (q.rank == 0 && tid == 0) write_choice(p, row, Choice{first, share_of(static_cast<uint64_t>(kWeightOne), total)});
   } else {
     const uint64_t unit = drawn_unit(uniform, total);
     ahead += sh.scan[warp];
@@ -1011,7 +1086,7 @@ __global__ void __launch_bounds__(kMaxThreads) choose_wide_kernel(ChooseParams p
         const uint64_t before = ahead + warp_exclusive_u64(w, lane);
         const bool here = w && unit >= before && unit < before + w;
         if (here)
-          write_choice(p, row, Choice{q.c0 + i, static_cast<float>(static_cast<double>(w) / static_cast<double>(total))});
+          write_choice(p, row, Choice{q.c0 + i, share_of(w, total)});
         ahead = __shfl_sync(~0u, before + w, 31);
         if (__any_sync(~0u, here)) break;
       }
