@@ -1,5 +1,4 @@
 // The policy operators; see policy.cuh for the arguments.
-#include <cooperative_groups.h>
 #include <type_traits>
 
 #include "kernels.cuh"
@@ -106,60 +105,93 @@ __global__ void __launch_bounds__(kThreads) slot_table_kernel(SlotTableParams p,
     fill_row<QUADS>(p, row, first[row - r0], first[row - r0 + 1] - first[row - r0], lane);
 }
 
-// Many rows: the sums come first, by one cluster of eight blocks that each take an eighth of the rows,
-// add them up, exchange the eight sums through distributed shared memory and then write `starts`.
-constexpr int kScanBlocks = 8;
+// Many rows, in three launches. The first adds up the lengths of each chunk of rows, the second turns
+// these sums into the chunks' starts, and the third lays the chunks out, a block each. A chunk's sum
+// waits in `starts` itself, behind its first row: nobody but that chunk's block reads or writes it later.
+constexpr int kChunkRows = 64;
 
-__global__ void __cluster_dims__(kScanBlocks, 1, 1) __launch_bounds__(1024) slot_starts_kernel(SlotTableParams p) {
-  __shared__ int sums[32];
-  __shared__ int mine;
-  grid_dep_wait();
-  grid_dep_launch();
-  cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
-  const int tid = threadIdx.x, rank = cluster.block_rank();
-  const int64_t per = (static_cast<int64_t>(p.rows) + kScanBlocks - 1) / kScanBlocks;
-  const int64_t r0 = min(rank * per, static_cast<int64_t>(p.rows)), r1 = min(r0 + per, static_cast<int64_t>(p.rows));
-  int sum = 0, total;
-  for (int64_t r = r0 + tid; r < r1; r += 1024) sum += clamped_length(p, static_cast<int>(r));
-  block_exclusive(sum, sums, &total);
-  if (tid == 0) mine = total;
-  cluster.sync();
-  int base = 0;
-  for (int q = 0; q < rank; ++q) base += *cluster.map_shared_rank(&mine, q);
-  cluster.sync();  // no block leaves while another reads its sum
-  for (int64_t c = r0; c < r1; c += 1024) {
-    const int64_t row = c + tid;
-    int n = 0;
-    if (row < r1) {
-      n = clamped_length(p, static_cast<int>(row));
-      if (n != p.lengths[row]) flag_length(p);
-    }
-    const int at = base + block_exclusive(n, sums, &total);
-    if (row < r1) p.starts[row] = at;
-    base += total;
-  }
-  if (rank == kScanBlocks - 1 && tid == 0) {
-    p.starts[p.rows] = base;
-    if (base > p.count) flag_length(p);
-  }
+__device__ __forceinline__ int32_t* chunk_sum(const SlotTableParams& p, int64_t chunk) {
+  return p.starts + chunk * kChunkRows + 1;
 }
 
-// Then every warp lays out `per` <= 32 rows, whose starts it reads at once.
-template <bool QUADS>
-__global__ void __launch_bounds__(kThreads) slot_fill_kernel(SlotTableParams p, int per) {
+__global__ void __launch_bounds__(kThreads) slot_sums_kernel(SlotTableParams p, int64_t chunks) {
   grid_dep_wait();
   grid_dep_launch();
   const int lane = threadIdx.x & 31;
-  const int64_t r0 = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * per;
-  if (r0 >= p.rows) return;
-  const int rows = static_cast<int>(min(static_cast<int64_t>(per), p.rows - r0));
-  const int here = lane < rows ? p.starts[r0 + lane] : 0, next = lane < rows ? p.starts[r0 + lane + 1] : 0;
-  for (int i = 0; i < rows; ++i) {
-    const int first = __shfl_sync(~0u, here, i);
-    fill_row<QUADS>(p, static_cast<int>(r0) + i, first, __shfl_sync(~0u, next, i) - first, lane);
+  const int64_t chunk = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  if (chunk >= chunks) return;
+  int sum = 0;
+#pragma unroll
+  for (int i = 0; i < kChunkRows / 32; ++i) {
+    const int64_t row = chunk * kChunkRows + 32 * i + lane;
+    if (row < p.rows) {
+      const int n = clamped_length(p, static_cast<int>(row));
+      if (n != p.lengths[row]) flag_length(p);
+      sum += n;
+    }
   }
+  sum = __reduce_add_sync(~0u, sum);
+  if (lane == 0) *chunk_sum(p, chunk) = sum;
 }
 
+__global__ void __launch_bounds__(1024) slot_starts_kernel(SlotTableParams p, int64_t chunks) {
+  __shared__ int sums[32];
+  grid_dep_wait();
+  grid_dep_launch();
+  constexpr int kRun = 4;  // chunks of a thread
+  int base = 0, total;
+  for (int64_t c0 = 0; c0 < chunks; c0 += 1024 * kRun) {
+    const int64_t c = c0 + static_cast<int64_t>(threadIdx.x) * kRun;
+    int v[kRun], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) v[i] = c + i < chunks ? *chunk_sum(p, c + i) : 0;
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) sum += v[i];
+    int at = base + block_exclusive(sum, sums, &total);
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      if (c + i < chunks) *chunk_sum(p, c + i) = at;
+      at += v[i];
+    }
+    base += total;
+  }
+  if (threadIdx.x == 0 && base > p.count) flag_length(p);
+}
+
+template <bool QUADS>
+__global__ void __launch_bounds__(kThreads) slot_fill_kernel(SlotTableParams p) {
+  __shared__ int first[kChunkRows + 1];
+  grid_dep_wait();
+  grid_dep_launch();
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kChunkRows;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(kChunkRows), p.rows - r0));
+  if (tid < 32) {
+    int at = *chunk_sum(p, blockIdx.x);
+    __syncwarp();  // read before it is overwritten
+#pragma unroll
+    for (int i = 0; i < kChunkRows / 32; ++i) {
+      const int r = 32 * i + lane;
+      const int n = r < rows ? clamped_length(p, static_cast<int>(r0 + r)) : 0;
+      int in = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(~0u, in, o);
+        if (lane >= o) in += u;
+      }
+      first[r] = at + in - n;
+      if (r < rows) p.starts[r0 + r] = at + in - n;
+      at += __shfl_sync(~0u, in, 31);
+    }
+    if (lane == 0) {
+      first[kChunkRows] = at;
+      if (r0 + rows == p.rows) p.starts[p.rows] = at;
+    }
+  }
+  __syncthreads();
+  for (int r = tid >> 5; r < rows; r += kWarps)
+    fill_row<QUADS>(p, static_cast<int>(r0) + r, first[r], first[r + 1] - first[r], lane);
+}
 
 // ---- narrow rows: one warp each ------------------------------------------------------------
 // A row of up to 512 columns (a slot row has 224) stays in the registers of one warp, column
@@ -171,7 +203,7 @@ constexpr int kNarrowWarps = 4;
 // full, so that a probe always ends), or a count for each column; then, for the choice, the columns
 // that are left.
 template <int K>
-struct NarrowShared {
+struct alignas(16) NarrowShared {
   static constexpr int kEntries = 64 * K;  // twice the columns, a power of two
   union {
     struct {
@@ -214,6 +246,18 @@ __device__ __forceinline__ void load_narrow(const LogitParams& p, int row, int l
   const T* logits = static_cast<const T*>(p.logits) + row * p.stride;
   const Penalties pen = row_penalties(r, row);
   const uint32_t* mask = r.mask ? r.mask + row * r.mask_stride : nullptr;
+  const int32_t* history = r.history + row * r.history_stride;
+  const int32_t* ids = r.bias_actions + row * r.bias_stride;
+  const float* values = r.bias_values + row * r.bias_stride;
+  const int biases = r.bias_len;
+  // Everything that the row reads first is asked for at once: the first of both lists, whether the row
+  // has that many entries or not, slots and logits.
+  constexpr int kAhead = 2;  // history entries of a lane
+  int seen[kAhead];
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) seen[u] = r.history && lane + 32 * u < r.history_len ? history[lane + 32 * u] : -1;
+  int id = lane < biases ? ids[lane] : -1;
+  float value = lane < biases ? values[lane] : 0.f;
   int a[K], at[K];  // the column's action, -1 where it is masked or empty; its count's place
 #pragma unroll
   for (int k = 0; k < K; ++k) {
@@ -225,6 +269,7 @@ __device__ __forceinline__ void load_narrow(const LogitParams& p, int row, int l
       v[k] = as_float(logits[c]);
     }
   }
+  unsigned used = 0;  // bit k: some lane's column 32 k + lane is left; lists of moves fill the first slots only
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     if (SLOTS && a[k] >= r.actions) {
@@ -233,12 +278,15 @@ __device__ __forceinline__ void load_narrow(const LogitParams& p, int row, int l
     }
     at[k] = 32 * k + lane;
     if (mask && a[k] >= 0 && !((mask[a[k] >> 5] >> (a[k] & 31)) & 1)) a[k] = -1;
+    if (__any_sync(~0u, a[k] >= 0)) used |= 1u << k;
   }
-  const int biases = r.bias_len;
   if (pen.seen > 0 || (SLOTS && biases)) {
     if (SLOTS) {
 #pragma unroll
-      for (int i = 0; i < 2 * K; ++i) sh.keys[32 * i + lane] = -1, sh.counts[32 * i + lane] = 0;
+      for (int i = 0; i < K / 2; ++i) {
+        reinterpret_cast<int4*>(sh.keys)[32 * i + lane] = make_int4(-1, -1, -1, -1);
+        reinterpret_cast<int4*>(sh.counts)[32 * i + lane] = make_int4(0, 0, 0, 0);
+      }
     } else {
 #pragma unroll
       for (int k = 0; k < K; ++k) sh.counts[32 * k + lane] = 0;
@@ -247,28 +295,31 @@ __device__ __forceinline__ void load_narrow(const LogitParams& p, int row, int l
     if (SLOTS) {
 #pragma unroll
       for (int k = 0; k < K; ++k)
-        if (a[k] >= 0) at[k] = sh.insert(a[k]);
+        if ((used >> k) & 1 && a[k] >= 0) at[k] = sh.insert(a[k]);
       __syncwarp();
     }
-    const int32_t* history = r.history + row * r.history_stride;
-    for (int e = lane; e < pen.seen; e += 32) {
-      const int id = history[e];
-      const int h = id < 0 ? -1 : SLOTS ? sh.find(id) : id < p.width ? id : -1;
+    auto count = [&](int action) {
+      const int h = action < 0 ? -1 : SLOTS ? sh.find(action) : action < p.width ? action : -1;
       if (h >= 0) atomicAdd(&sh.counts[h], 1);
-    }
+    };
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (lane + 32 * u < pen.seen) count(seen[u]);
+    for (int e = lane + 32 * kAhead; e < pen.seen; e += 32) count(history[e]);
     __syncwarp();
     if (pen.seen > 0) {
 #pragma unroll
       for (int k = 0; k < K; ++k)
-        if (a[k] >= 0) v[k] = penalised(v[k], sh.counts[at[k]], pen);
+        if ((used >> k) & 1 && a[k] >= 0) v[k] = penalised(v[k], sh.counts[at[k]], pen);
     }
   }
   // Biases in the list's order: every lane looks one entry up, and the ones that name a column are
   // added one after the other.
   for (int e0 = 0; e0 < biases; e0 += 32) {
-    const int e = e0 + lane;
-    const int id = e < biases ? r.bias_actions[row * r.bias_stride + e] : -1;
-    const float value = e < biases ? r.bias_values[row * r.bias_stride + e] : 0.f;
+    if (e0) {
+      id = e0 + lane < biases ? ids[e0 + lane] : -1;
+      value = e0 + lane < biases ? values[e0 + lane] : 0.f;
+    }
     const int h = id < 0 ? -1 : SLOTS ? sh.find(id) : id < p.width ? id : -1;
     unsigned todo = __ballot_sync(~0u, h >= 0);
     while (todo) {
@@ -496,13 +547,14 @@ cudaError_t launch_slot_table(const SlotTableParams& p, cudaStream_t s) {
     return launch_kernel(quads ? slot_table_kernel<true> : slot_table_kernel<false>, dim3(blocks), dim3(kThreads), 0, s, p,
                          per);
   }
-  const cudaError_t e = launch_kernel(slot_starts_kernel, dim3(kScanBlocks), dim3(1024), 0, s, p);
+  const int64_t chunks = (static_cast<int64_t>(p.rows) + kChunkRows - 1) / kChunkRows;
+  cudaError_t e = launch_kernel(slot_sums_kernel, dim3(static_cast<unsigned>((chunks + kWarps - 1) / kWarps)), dim3(kThreads), 0,
+                                s, p, chunks);
   if (e != cudaSuccess) return e;
-  const PdlScope pdl(true);  // the second kernel waits for the first before it reads `starts`
-  const int per = 8;
-  const int64_t warps = (static_cast<int64_t>(p.rows) + per - 1) / per;
-  return launch_kernel(quads ? slot_fill_kernel<true> : slot_fill_kernel<false>,
-                       dim3(static_cast<unsigned>((warps + kWarps - 1) / kWarps)), dim3(kThreads), 0, s, p, per);
+  const PdlScope pdl(true);  // each waits for the one before it to finish before it reads anything
+  if ((e = launch_kernel(slot_starts_kernel, dim3(1), dim3(1024), 0, s, p, chunks)) != cudaSuccess) return e;
+  return launch_kernel(quads ? slot_fill_kernel<true> : slot_fill_kernel<false>, dim3(static_cast<unsigned>(chunks)),
+                       dim3(kThreads), 0, s, p);
 }
 
 cudaError_t launch_adjust(const AdjustParams& p, cudaStream_t s) {
@@ -524,6 +576,7 @@ cudaError_t launch_choose(const ChooseParams& p, cudaStream_t s) {
 cudaError_t prepare_policy() {
   cudaFuncAttributes a;
   cudaError_t e;
+  if ((e = cudaFuncGetAttributes(&a, slot_sums_kernel)) != cudaSuccess) return e;
   if ((e = cudaFuncGetAttributes(&a, slot_starts_kernel)) != cudaSuccess) return e;
   if ((e = cudaFuncGetAttributes(&a, slot_fill_kernel<true>)) != cudaSuccess) return e;
   if ((e = cudaFuncGetAttributes(&a, slot_fill_kernel<false>)) != cudaSuccess) return e;
