@@ -239,9 +239,10 @@ struct alignas(16) NarrowShared {
   }
 };
 
-// Adjusted logits of a row.
+// Adjusted logits of a row. Returns the k whose columns are not all masked or empty, a bit each: lists of
+// moves fill the first slots only, and what follows can pass over the rest.
 template <class T, int K, bool SLOTS>
-__device__ __forceinline__ void load_narrow(const LogitParams& p, int row, int lane, NarrowShared<K>& sh, float (&v)[K]) {
+__device__ __forceinline__ unsigned load_narrow(const LogitParams& p, int row, int lane, NarrowShared<K>& sh, float (&v)[K]) {
   const RuleParams& r = p.rules;
   const T* logits = static_cast<const T*>(p.logits) + row * p.stride;
   const Penalties pen = row_penalties(r, row);
@@ -269,7 +270,7 @@ __device__ __forceinline__ void load_narrow(const LogitParams& p, int row, int l
       v[k] = as_float(logits[c]);
     }
   }
-  unsigned used = 0;  // bit k: some lane's column 32 k + lane is left; lists of moves fill the first slots only
+  unsigned used = 0;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     if (SLOTS && a[k] >= r.actions) {
@@ -335,6 +336,7 @@ __device__ __forceinline__ void load_narrow(const LogitParams& p, int row, int l
 #pragma unroll
   for (int k = 0; k < K; ++k)
     if (a[k] < 0) v[k] = -INFINITY;
+  return used;
 }
 
 template <class T, int K, bool SLOTS>
@@ -347,7 +349,7 @@ __global__ void __launch_bounds__(kNarrowWarps * 32) adjust_narrow_kernel(Adjust
   if (row >= p.in.rows) return;
   const int width = p.in.width;
   float v[K];
-  load_narrow<T, K, SLOTS>(p.in, row, lane, shared[warp], v);
+  const unsigned used = load_narrow<T, K, SLOTS>(p.in, row, lane, shared[warp], v);
   if (p.out) {
     T* out = static_cast<T*>(p.out) + row * p.out_stride;
 #pragma unroll
@@ -357,36 +359,46 @@ __global__ void __launch_bounds__(kNarrowWarps * 32) adjust_narrow_kernel(Adjust
   if (!p.priors) return;
   const float t = p.in.temperature ? p.in.temperature[row] : 1.f;
   float m = -INFINITY;
-  bool nan = t != t;
 #pragma unroll
-  for (int k = 0; k < K; ++k) m = fmaxf(m, v[k]), nan |= v[k] != v[k];
-  m = warp_max(m);
-  nan = __any_sync(~0u, nan);
+  for (int k = 0; k < K; ++k)
+    if ((used >> k) & 1) m = max_or_nan(m, v[k]);
+  m = warp_max_or_nan(m);
   float* priors = p.priors + row * p.priors_stride;
-  float e[K];
-  if (t <= 0.f && !nan) {  // the lowest column of the largest logit
-    int first = kPolicyMaxWidth;
-#pragma unroll
-    for (int k = K - 1; k >= 0; --k)
-      if (v[k] == m && m > -INFINITY) first = 32 * k + lane;
-    first = __reduce_min_sync(~0u, first);
-#pragma unroll
-    for (int k = 0; k < K; ++k) e[k] = 32 * k + lane == first ? 1.f : 0.f;
-  } else {
-    float sum = 0.f;
+  float sum = 0.f, inv;
+  if (m > -INFINITY && m < INFINITY && t > 0.f) {
+    const float scale = exponent_scale(t);  // exp((v - m) / t)
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      e[k] = v[k] == -INFINITY ? 0.f : v[k] == m ? 1.f : m == INFINITY ? 0.f : expf((v[k] - m) / t);
-      sum += e[k];
+      float e = 0.f;
+      if ((used >> k) & 1) e = power_of_two((v[k] - m) * scale);
+      v[k] = e;
+      sum += e;
+    }
+    inv = 1.f / warp_sum(sum);
+  } else {
+    // Nothing left: 0. A NaN, in the row or as t: NaN wherever something is left. Else the largest
+    // logit's lowest column, or the columns at +inf.
+    const bool nan = m != m || t != t;
+    int first = -1;
+    if (!nan && t <= 0.f) {
+      first = kPolicyMaxWidth;
+#pragma unroll
+      for (int k = K - 1; k >= 0; --k)
+        if (v[k] == m) first = 32 * k + lane;
+      first = __reduce_min_sync(~0u, first);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const bool there = v[k] == m && (t > 0.f || 32 * k + lane == first);
+      v[k] = v[k] == -INFINITY ? 0.f : nan ? NAN : there ? 1.f : 0.f;
+      if (!nan) sum += v[k];
     }
     sum = warp_sum(sum);
-    const float inv = nan ? NAN : sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-    for (int k = 0; k < K; ++k) e[k] = v[k] == -INFINITY ? 0.f : e[k] * inv;
+    inv = sum == 0.f ? 1.f : 1.f / sum;
   }
 #pragma unroll
   for (int k = 0; k < K; ++k)
-    if (32 * k + lane < width) priors[32 * k + lane] = e[k];
+    if (32 * k + lane < width) priors[32 * k + lane] = v[k] * inv;
 }
 
 // Draws from the `left` <= 32 G columns in sh.x, which are in column order. With a cut-off they are
@@ -472,15 +484,15 @@ __global__ void __launch_bounds__(kNarrowWarps * 32) choose_narrow_kernel(Choose
   if (row >= p.in.rows) return;
   NarrowShared<K>& sh = shared[warp];
   float v[K];
-  load_narrow<T, K, SLOTS>(p.in, row, lane, sh, v);
+  const unsigned used = load_narrow<T, K, SLOTS>(p.in, row, lane, sh, v);
   __syncwarp();
   const float t = p.in.temperature ? p.in.temperature[row] : 1.f;
   float m = -INFINITY;
-  bool nan = t != t;
   int left = 0;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    m = fmaxf(m, v[k]), nan |= v[k] != v[k];
+    if (!((used >> k) & 1)) continue;
+    m = max_or_nan(m, v[k]);
     const unsigned here = __ballot_sync(~0u, v[k] > -INFINITY);
     if (v[k] > -INFINITY) {
       const int i = left + __popc(here & ((1u << lane) - 1));
@@ -488,8 +500,8 @@ __global__ void __launch_bounds__(kNarrowWarps * 32) choose_narrow_kernel(Choose
     }
     left += __popc(here);
   }
-  m = warp_max(m);
-  nan = __any_sync(~0u, nan);
+  m = warp_max_or_nan(m);
+  const bool nan = m != m || t != t;
   __syncwarp();
   Choice c{-1, nan ? NAN : 0.f};
   if (!nan && left) {

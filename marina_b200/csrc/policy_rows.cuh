@@ -48,6 +48,31 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   return u ^ (static_cast<uint32_t>(static_cast<int>(u) >> 31) | 0x80000000u);
 }
 
+// The larger of two, NaN if one is.
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+__device__ __forceinline__ float warp_max_or_nan(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = max_or_nan(v, __shfl_xor_sync(~0u, v, o));
+  return v;
+}
+
+__device__ __forceinline__ float power_of_two(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// log2(e) / t for t > 0, kept finite and above 0: with it (x - m) * scale is 0 for x = m and -inf for
+// x = -inf at every temperature, infinite ones and the smallest included.
+__device__ __forceinline__ float exponent_scale(float t) {
+  return fmaxf(fminf(1.44269504088896341f / t, 3.4e38f), 1.5e-45f);
+}
+
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }

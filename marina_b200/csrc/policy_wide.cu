@@ -287,7 +287,7 @@ __device__ __forceinline__ uint32_t row_best(const Part& q, const float (&x)[kQu
 #pragma unroll
   for (int k = 0; k < kQuads; ++k)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(x[k][j]));
+    for (int j = 0; j < 4; ++j) m = max_or_nan(m, x[k][j]);
   const uint32_t key = m != m ? ~0u : m == -INFINITY ? 0u : order_key(m);
   return row_reduce(q, key, [](uint32_t a, uint32_t b) { return a > b ? a : b; }, ex);
 }
@@ -302,12 +302,6 @@ __device__ __forceinline__ int row_first(const Part& q, const float (&x)[kQuads]
     for (int j = 3; j >= 0; --j)
       if (x[k][j] == m) first = min(first, q.c0 + span_base(k) + span_column<QUADS>(j));
   return row_reduce(q, first, [](int a, int b) { return a < b ? a : b; }, ex);
-}
-
-__device__ __forceinline__ float power_of_two(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
 }
 
 // Bound by HBM: a logit is read once, stays in a register through maximum, exponential and sum, and
@@ -336,8 +330,7 @@ __global__ void __launch_bounds__(kMaxThreads) adjust_wide_kernel(AdjustParams p
   float sum = 0.f, inv;
   auto total = [&]() { return row_reduce(q, sum, [](float a, float b) { return a + b; }, ex_sum); };
   if (best && best != ~0u && t > 0.f && m != INFINITY) {
-    // exp((x - m) / t). The scale is finite and not 0, so that 0 stays 0 and -inf stays -inf under it.
-    const float scale = fmaxf(fminf(1.44269504088896341f / t, 3.4e38f), 1.5e-45f);
+    const float scale = exponent_scale(t);  // exp((x - m) / t)
 #pragma unroll
     for (int k = 0; k < kQuads; ++k)
 #pragma unroll
