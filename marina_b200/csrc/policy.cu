@@ -198,6 +198,7 @@ __global__ void __launch_bounds__(kThreads) slot_fill_kernel(SlotTableParams p) 
 // 32 k + lane in v[k]: nothing but warp shuffles between its steps, and every global read of the row
 // in flight at once. COLUMNS = K * 32 is the widest row of an instantiation.
 constexpr int kNarrowWarps = 4;
+constexpr int kCompared = 128;  // longest lists that are compared with a row's columns entry by entry
 
 // A warp's shared memory: a hash table from action to count (for slots; linear probing, at most half
 // full, so that a probe always ends), or a count for each column; then, for the choice, the columns
@@ -280,6 +281,49 @@ __device__ __forceinline__ unsigned load_narrow(const LogitParams& p, int row, i
     at[k] = 32 * k + lane;
     if (mask && a[k] >= 0 && !((mask[a[k] >> 5] >> (a[k] & 31)) & 1)) a[k] = -1;
     if (__any_sync(~0u, a[k] >= 0)) used |= 1u << k;
+  }
+  if (SLOTS && pen.seen <= kCompared && biases <= kCompared) {
+    // Short lists: every entry is shown to the columns of every lane, of which rows of up to 64 moves
+    // have two. Measured on 8192 rows of 224 slots, 40 entries and 8 biases: 12.6 us, and 15.3 us with the
+    // hash table, whose insertions take 7 us in the longest rows.
+    auto compare = [&](auto columns) {
+      constexpr int C = decltype(columns)::value;
+      if (pen.seen > 0) {
+        int c[C] = {};
+        for (int e0 = 0; e0 < pen.seen; e0 += 32) {
+          const int mine = e0 == 0 ? seen[0] : e0 == 32 ? seen[1] : e0 + lane < pen.seen ? history[e0 + lane] : -1;
+          const int count = min(32, pen.seen - e0);
+          for (int e = 0; e < count; ++e) {
+            const int action = __shfl_sync(~0u, mine, e);
+#pragma unroll
+            for (int k = 0; k < C; ++k) c[k] += action == a[k];
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < C; ++k)
+          if (a[k] >= 0) v[k] = penalised(v[k], c[k], pen);
+      }
+      for (int e0 = 0; e0 < biases; e0 += 32) {
+        if (e0) {
+          id = e0 + lane < biases ? ids[e0 + lane] : -1;
+          value = e0 + lane < biases ? values[e0 + lane] : 0.f;
+        }
+        const int count = min(32, biases - e0);
+        for (int e = 0; e < count; ++e) {
+          const int action = __shfl_sync(~0u, id, e);
+          const float add = __shfl_sync(~0u, value, e);
+#pragma unroll
+          for (int k = 0; k < C; ++k)
+            if (action == a[k]) v[k] = __fadd_rn(v[k], add);
+        }
+      }
+    };
+    if (used < 4) compare(std::integral_constant<int, 2>());
+    else compare(std::integral_constant<int, K>());
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (a[k] < 0) v[k] = -INFINITY;
+    return used;
   }
   if (pen.seen > 0 || (SLOTS && biases)) {
     if (SLOTS) {
