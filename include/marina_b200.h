@@ -265,7 +265,9 @@ MRN_API int mrn_evaluate_device_static(mrn_ctx* ctx, int n, const uint8_t* d_boa
  * was. Nothing orders these calls with work on other streams, the context's passes included: that
  * is the caller's, with events. Outputs must not overlap inputs or one another, except where it
  * says so. Numbers on the device cannot be refused by the call: what a bad one does is said with
- * the argument, and none of them makes a kernel read or write outside the buffers. */
+ * the argument, and none of them makes a kernel read or write outside the buffers. Some set the
+ * context's status word, which mrn_status_word reads and clears; the next synchronous call on the
+ * context fails with it otherwise. */
 
 /* Element type of logits. */
 typedef enum mrn_type {
@@ -277,6 +279,8 @@ typedef enum mrn_type {
 /* Columns a row of mrn_adjust_logits and mrn_choose_actions may have, and rows of a call. */
 #define MRN_MAX_WIDTH (1 << 18)
 #define MRN_MAX_ROWS (1 << 27)
+/* Entries of a row's history and of its bias list. */
+#define MRN_MAX_LIST (1 << 20)
 
 /* What changes the logits of a batch of rows. Strides count elements between rows; a stride of 0
  * makes every row share one list. Unused parts are NULL (or have length 0).

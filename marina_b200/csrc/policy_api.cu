@@ -52,6 +52,9 @@ int rule_params(mrn_ctx* c, int rows, int width, const mrn_rules* r, RuleParams*
                    (long long)words);
   if (r->bias_len < 0 || r->history_len < 0)
     return c->fail(MRN_ERR_ARGUMENT, "rules: a negative length (bias_len %d, history_len %d)", r->bias_len, r->history_len);
+  if (r->bias_len > MRN_MAX_LIST || r->history_len > MRN_MAX_LIST)
+    return c->fail(MRN_ERR_ARGUMENT, "rules: a list longer than %d (bias_len %d, history_len %d)", MRN_MAX_LIST, r->bias_len,
+                   r->history_len);
   if (r->bias_len && (!r->bias_actions || !r->bias_values))
     return c->fail(MRN_ERR_ARGUMENT, "rules: bias_len %d without bias_actions and bias_values", r->bias_len);
   if (r->bias_len && (r->bias_stride < 0 || (r->bias_stride > 0 && r->bias_stride < r->bias_len)))
@@ -137,6 +140,15 @@ MRN_API int mrn_slot_table(mrn_ctx* c, int rows, int width, const int32_t* lengt
   if (!starts || (rows && (!lengths || !table)) || (count && !entries)) return c->fail(MRN_ERR_ARGUMENT, "NULL buffer");
   for (const void* p : {(const void*)lengths, (const void*)entries, (const void*)starts, (const void*)table, (const void*)map})
     if (mrn::misaligned(p, 4)) return c->fail(MRN_ERR_ARGUMENT, "slot table: a pointer is not aligned to 4 bytes");
+  auto block = [](const void* p, int64_t elements) { return mrn::Block{elements ? p : nullptr, 0, elements * 4, 1}; };
+  const mrn::Block in[] = {block(lengths, rows), block(entries, count)};
+  const mrn::Block out[] = {block(starts, int64_t(rows) + 1), block(table, int64_t(rows) * width), block(map, count)};
+  for (int i = 0; i < 3; ++i) {
+    for (const mrn::Block& b : in)
+      if (mrn::overlap(out[i], b)) return c->fail(MRN_ERR_ARGUMENT, "slot table: an output overlaps an input");
+    for (int j = 0; j < i; ++j)
+      if (mrn::overlap(out[i], out[j])) return c->fail(MRN_ERR_ARGUMENT, "slot table: two outputs overlap");
+  }
   const mrn::DeviceScope device(c->device);
   if (device.error != cudaSuccess) return mrn::launched(c, device.error, "cudaSetDevice");
   const mrn::SlotTableParams p{rows, width, lengths, count, entries, starts, table, map, c->status};

@@ -54,14 +54,20 @@ def test_null_context():
     assert lib.mrn_choose_actions(None, 1, 1, P, 0, 1, None, None, None, None, None, Q, None, None, None) == 1
 
 
+SLOTS = dict(rows=4, width=224, lengths_ptr=P, count=9, entries_ptr=P, starts_ptr=Q, table_ptr=Q + 20, map_ptr=FAR)
+
+
 @pytest.mark.parametrize("change,words", [
+    ({"starts_ptr": P + 12}, "overlaps an input"), ({"map_ptr": P + 32}, "overlaps an input"),
+    ({"table_ptr": P - 4 * 224 * 4 + 4}, "overlaps an input"), ({"table_ptr": Q + 16}, "two outputs"),
+    ({"map_ptr": Q + 20}, "two outputs"),
     ({"rows": -1}, "rows -1"), ({"width": 0}, "width 0"), ({"count": -1}, "count -1"),
     ({"rows": 1 << 20, "width": 1 << 11}, "2^31 - 1"), ({"lengths_ptr": None}, "NULL"), ({"entries_ptr": None}, "NULL"),
     ({"starts_ptr": None}, "NULL"), ({"table_ptr": None}, "NULL"), ({"map_ptr": P + 2}, "aligned"),
     ({"lengths_ptr": P + 1}, "aligned"),
 ])
 def test_slot_table_refuses(net, change, words):
-    good = dict(rows=4, width=224, lengths_ptr=P, count=9, entries_ptr=P, starts_ptr=Q, table_ptr=Q, map_ptr=Q)
+    good = SLOTS
     reaches_the_device(lambda: net.slot_table(**good))
     refused(lambda: net.slot_table(**{**good, **change}), words)
 
@@ -74,7 +80,8 @@ BAD_RULES = [
     ({"actions": 0}, "actions 0"), ({"columns": None, "actions": 200}, "200 actions for 224 columns"),
     ({"columns_stride": 223}, "columns_stride 223"), ({"columns_stride": -1}, "columns_stride -1"),
     ({"mask_stride": 145}, "mask_stride 145"), ({"mask_stride": -146}, "mask_stride"), ({"bias_len": -1}, "negative"),
-    ({"history_len": -2}, "negative"), ({"bias_actions": None}, "bias_actions"), ({"bias_values": None}, "bias_values"),
+    ({"history_len": -2}, "negative"), ({"bias_len": (1 << 20) + 1}, "longer than 1048576"),
+    ({"history_len": (1 << 20) + 1, "history_stride": 1 << 21}, "longer than 1048576"), ({"bias_actions": None}, "bias_actions"), ({"bias_values": None}, "bias_values"),
     ({"bias_stride": 2}, "bias_stride 2"), ({"history": None}, "without history"), ({"history_stride": 4}, "history_stride 4"),
     *[({name: P + 2}, "aligned") for name in ("columns", "mask", "bias_actions", "bias_values", "history", "history_lens",
                                               "repetition", "presence", "frequency")],
