@@ -181,7 +181,7 @@ int run_moves(mrn_ctx* c, const MovesCall& m) {
   CK(mrn::launch_slot_table(table, s));
   CK(cudaGraphLaunch(b->slot_graph, s));
   const mrn::LogitParams in{c->slot_logits, mrn::LogitType::kF32, MRN_MAX_LEGAL, n, MRN_MAX_LEGAL, rules,
-                            static_cast<const float*>(per_row[4].on_device), c->status, c->num_sms};
+                            static_cast<const float*>(per_row[4].on_device), c->status};
   if (m.move) {
     const mrn::ChooseParams choose{in, static_cast<const int32_t*>(per_row[5].on_device),
                                    static_cast<const float*>(per_row[6].on_device),

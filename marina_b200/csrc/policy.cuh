@@ -42,7 +42,6 @@ struct LogitParams {
   RuleParams rules;
   const float* temperature;  // [rows], or null for 1
   int* status;               // device error word
-  int sms;                   // multiprocessors of the device
 };
 
 // Rows of one call: every row may take eight blocks of a grid.

@@ -95,7 +95,7 @@ int logit_params(mrn_ctx* c, int rows, int width, const void* logits, int type, 
   if (misaligned(logits, type == MRN_TYPE_F32 ? 4 : 2) || misaligned(temperature, 4))
     return c->fail(MRN_ERR_ARGUMENT, "logits or temperature is not aligned to its elements");
   out->logits = logits, out->type = static_cast<LogitType>(type), out->stride = stride;
-  out->rows = rows, out->width = width, out->temperature = temperature, out->status = c->status, out->sms = c->num_sms;
+  out->rows = rows, out->width = width, out->temperature = temperature, out->status = c->status;
   return rule_params(c, rows, width, rules, &out->rules);
 }
 

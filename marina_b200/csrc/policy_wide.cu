@@ -2,7 +2,6 @@
 // each block a contiguous segment of its columns, which it reads once into registers. Blocks of a row
 // exchange maxima, sums and histograms through distributed shared memory.
 #include <cooperative_groups.h>
-#include <stdlib.h>
 
 #include <type_traits>
 #include <utility>
@@ -305,7 +304,11 @@ __device__ __forceinline__ int row_first(const Part& q, const float (&x)[kQuads]
 }
 
 // Bound by HBM: a logit is read once, stays in a register through maximum, exponential and sum, and
-// leaves as its adjusted value and its prior.
+// leaves as its adjusted value and its prior. 4096 rows of 4672 f32 without lists take 37.9 us (6.1 TB/s of
+// the 6.57 measured for a copy), with a history of 40 entries and 16 biases 46.3 us (5.0 TB/s): what a list
+// names is looked up in shared memory between two barriers, and the row's other columns wait. 100 rows of
+// 100003 f16 under a mask: 12.4 us without lists, 36.5 us with histories of 4096 and 300 biases, which
+// every block of a row goes through.
 template <class T, bool QUADS>
 __global__ void __launch_bounds__(kMaxThreads) adjust_wide_kernel(AdjustParams p, int blocks, int segment) {
   extern __shared__ __align__(16) float cells[];
@@ -376,6 +379,8 @@ __global__ void __launch_bounds__(kMaxThreads) adjust_wide_kernel(AdjustParams p
 // even the bin holds more than the list; and the draw goes over the whole row again.
 constexpr int kBins = 512;
 constexpr float kBinsPerUnit = 18.f;  // exp(-512 / 18) < 2^-41: what lies below weighs 0
+// Measured with and without the short way: 61.0 and 77.6 us for 2048 rows of 4672, 15.4 and 47.0 us for one
+// row of 131072.
 constexpr int kFew = 256;
 
 __host__ __device__ constexpr int list_capacity(int segment) { return segment <= 8192 ? 1024 : 4096; }
@@ -987,6 +992,11 @@ __device__ __forceinline__ void draw_few(const ChooseParams& p, int row, const u
   }
 }
 
+// Bound by the latency of its steps, each a pass over shared memory between barriers, and by instruction
+// fetches (ncu: no_instruction and barrier are the first stalls): loops over shared memory are faster here
+// than the same work unrolled over registers, whose code does not stay in the cache. 2048 rows of 4672 f32
+// under a mask, top_k and top_p: 54 us; one row of 131072 bf16, top_k: 15.4 us; 64 rows of 150001 bf16 under
+// a mask, top_p alone: 118 us, for which one block of 608 threads fits a multiprocessor.
 template <class T, bool QUADS>
 __global__ void __launch_bounds__(kMaxThreads) choose_wide_kernel(ChooseParams p, int blocks, int segment) {
   extern __shared__ __align__(16) unsigned char dynamic[];
@@ -1025,7 +1035,10 @@ __global__ void __launch_bounds__(kMaxThreads) choose_wide_kernel(ChooseParams p
   if (k <= 0) mem.left = compact(q, mem.x, weight, segment, mem.places, sh);
   if (k > 0 || top_p < 1.f) {
     Border border{q, mem, sh, weight, m, kBinsPerUnit / t};
-    const bool small = k > 0 && border.few_k(mine, k);
+    // Under a mask the threads' maxima say little about the few columns that are left: all are counted.
+    // Rows of 4672 of which one column in 16 is left: 54.1 us per 2048 so and 61.0 by the maxima; one row
+    // of 131072 without a mask: 19.2 and 15.4 us.
+    const bool small = k > 0 && !p.in.rules.mask && border.few_k(mine, k);
     if (!small && k > 0) mem.left = compact(q, mem.x, weight, segment, mem.places, sh);
     if (small || border.few(k, top_p)) {
       if (q.rank == 0)
@@ -1088,21 +1101,21 @@ __global__ void __launch_bounds__(kMaxThreads) choose_wide_kernel(ChooseParams p
   if (q.blocks > 1) cg::this_cluster().sync();  // no block leaves while another reads from it
 }
 
+constexpr int kWholeRow = 16384;
+
 struct Shape {
   int blocks, segment, threads;
 };
 
-// Blocks per row: enough for segments of 8192 columns, and more where the rows alone would leave
-// multiprocessors idle, as long as a segment keeps 1024 columns. Threads: as many as hold the segment.
+// Blocks per row, and threads: as many as hold the segment. A row of up to 16384 columns is one block's
+// even where that leaves multiprocessors idle, as what blocks exchange costs more than they save (us,
+// adjust / choose, 1 row of 4672: 5.2 / 8.8 by one block, 6.3 / 10.2 by two; 512 rows of 16000: 22.2 / 44.9
+// and 24.4 / 41.8). Above, blocks take 8192 columns each (128 rows of 60000: 24.6 / 38.0 by eight blocks,
+// 25.5 / 49.9 by four), or an eighth of the row.
 Shape wide_shape(const LogitParams& p) {
   const int width = p.width;
   int blocks = 1;
-  while (blocks < kMaxBlocks &&
-         (width > blocks * 8192 || (static_cast<int64_t>(p.rows) * blocks < p.sms && width >= blocks * 2048)))
-    blocks *= 2;
-#ifdef MRN_TUNE
-  if (getenv("MRN_B")) blocks = atoi(getenv("MRN_B"));
-#endif
+  while (width > kWholeRow && blocks < kMaxBlocks && width > blocks * 8192) blocks *= 2;
   Shape s;
   s.blocks = blocks;
   s.segment = ((width + blocks - 1) / blocks + kSpan - 1) / kSpan * kSpan;
