@@ -43,29 +43,52 @@ __device__ __forceinline__ void flag_length(const SlotTableParams& p) {
   if (p.status) atomicCAS(p.status, 0, kErrBadLength);
 }
 
-// One row of the table and the map, by one warp: table[r, s] = entries[first + s] for s < n, -1
-// behind; map[first + s] = r * width + s. QUADS: rows are 16-byte aligned, four slots to a store.
-template <bool QUADS>
-__device__ __forceinline__ void fill_row(const SlotTableParams& p, int row, int first, int n, int lane) {
-  const int at = row * p.width;  // rows * width < 2^31
-  const int listed = min(n, p.count - first);  // <= 0 where the entries ended before
+// ROWS rows of the table and the map, by one warp: table[r, s] = entries[first + s] for s < n, -1 behind;
+// map[first + s] = r * width + s. The rows' entries are asked for together. QUADS: rows are 16-byte
+// aligned, four slots to a store.
+template <bool QUADS, int ROWS>
+__device__ __forceinline__ void fill_rows(const SlotTableParams& p, const int (&row)[ROWS], const int (&first)[ROWS],
+                                          const int (&n)[ROWS], int lane) {
+  int listed[ROWS];  // <= 0 where the entries ended before, or there is no such row
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) listed[i] = min(n[i], p.count - first[i]);
   if (QUADS) {
     for (int s = 4 * lane; s < p.width; s += 128) {
-      int4 v = make_int4(-1, -1, -1, -1);
-      if (s < listed) v.x = __ldg(p.entries + first + s);
-      if (s + 1 < listed) v.y = __ldg(p.entries + first + s + 1);
-      if (s + 2 < listed) v.z = __ldg(p.entries + first + s + 2);
-      if (s + 3 < listed) v.w = __ldg(p.entries + first + s + 3);
-      *reinterpret_cast<int4*>(p.table + at + s) = v;
+      int4 v[ROWS];
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        const int32_t* from = p.entries + first[i] + s;
+        v[i].x = s < listed[i] ? __ldg(from) : -1;
+        v[i].y = s + 1 < listed[i] ? __ldg(from + 1) : -1;
+        v[i].z = s + 2 < listed[i] ? __ldg(from + 2) : -1;
+        v[i].w = s + 3 < listed[i] ? __ldg(from + 3) : -1;
+      }
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i)
+        if (row[i] < p.rows) {
+          int4* to = reinterpret_cast<int4*>(p.table + row[i] * p.width + s);
+          if (ROWS > 1) __stcs(to, v[i]);  // a large table does not stay in L2 anyway (65.2 -> 63.5 us)
+          else *to = v[i];
+        }
     }
   } else {
-    for (int s = lane; s < p.width; s += 32) p.table[at + s] = s < listed ? __ldg(p.entries + first + s) : -1;
+    for (int s = lane; s < p.width; s += 32) {
+      int v[ROWS];
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) v[i] = s < listed[i] ? __ldg(p.entries + first[i] + s) : -1;
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i)
+        if (row[i] < p.rows) p.table[row[i] * p.width + s] = v[i];
+    }
   }
-  if (p.map)
-    for (int s = lane; s < listed; s += 32) p.map[first + s] = at + s;
+  if (p.map) {
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i)
+      for (int s = lane; s < listed[i]; s += 32) p.map[first[i] + s] = row[i] * p.width + s;
+  }
 }
 
-// Bound by HBM where there are many rows (262144 rows of 224: 67.8 us, 4.7 TB/s of the 6.57 measured for a
+// Bound by HBM where there are many rows (262144 rows of 224: 63.5 us, 5.0 TB/s of the 6.57 measured for a
 // copy), by the launch where there are few (4096 rows: 4.0 us).
 //
 // Few rows: one launch. Block b lays out the rows [b * per, (b + 1) * per), per <= 32, and finds where
@@ -105,8 +128,8 @@ __global__ void __launch_bounds__(kThreads) slot_table_kernel(SlotTableParams p,
     }
   }
   __syncthreads();
-  for (int row = r0 + (tid >> 5); row < r1; row += kWarps)
-    fill_row<QUADS>(p, row, first[row - r0], first[row - r0 + 1] - first[row - r0], lane);
+  for (int r = tid >> 5; r0 + r < r1; r += kWarps)
+    fill_rows<QUADS, 1>(p, {r0 + r}, {first[r]}, {first[r + 1] - first[r]}, lane);
 }
 
 // Many rows, in three launches. The first adds up the lengths of each chunk of rows, the second turns
@@ -193,8 +216,18 @@ __global__ void __launch_bounds__(kThreads) slot_fill_kernel(SlotTableParams p) 
     }
   }
   __syncthreads();
-  for (int r = tid >> 5; r < rows; r += kWarps)
-    fill_row<QUADS>(p, static_cast<int>(r0) + r, first[r], first[r + 1] - first[r], lane);
+  constexpr int kTogether = 4;  // rows of a warp: 65.2 us for 262144 rows of 224; one at a time 67.8, eight 75.1
+  for (int r = tid >> 5; r < rows; r += kTogether * kWarps) {
+    int row[kTogether], from[kTogether], n[kTogether];
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {
+      const int q = r + i * kWarps;
+      row[i] = q < rows ? static_cast<int>(r0) + q : p.rows;  // behind the last: not written
+      from[i] = q < rows ? first[q] : 0;
+      n[i] = q < rows ? first[q + 1] - first[q] : 0;
+    }
+    fill_rows<QUADS, kTogether>(p, row, from, n, lane);
+  }
 }
 
 // ---- narrow rows: one warp each ------------------------------------------------------------
