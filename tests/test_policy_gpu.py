@@ -720,3 +720,50 @@ def test_the_context_s_own_stream_and_the_callers_device(net):
     torch.cuda.synchronize()
     check_state(s)
     assert torch.cuda.current_device() == 0
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("width", [224, 513, 4672, 20011])
+def test_cutoffs_around_the_short_way(net, width, masked):
+    """top_k on both sides of what one warp or block draws from, and top_p alone over equal logits."""
+    rng = np.random.default_rng(width + 7)
+    ks = [1, 2, 31, 32, 33, 64, 65, 127, 128, 129, 255, 256, 257, 400]
+    rows = len(ks)
+    x = some_logits(rng, rows, width, "f32")
+    rules = Rules(width, mask=rng.random((rows, width)) < 0.3) if masked else None
+    u, k = rng.random(rows).astype(np.float32), np.array(ks, np.int32)
+    t = (0.4 + 2 * rng.random(rows)).astype(np.float32)
+    check_choose(net, x, rules, t, k, None, u)
+    check_choose(net, x, rules, t, k, rng.random(rows).astype(np.float32), u)
+    few = torch.from_numpy(rng.integers(0, 3, (rows, width)).astype(np.float32)).to("cuda:0")
+    few[0] = -2.5
+    check_choose(net, few, rules, None, None, rng.random(rows).astype(np.float32), u)
+    check_choose(net, few, rules, t, k, rng.random(rows).astype(np.float32), u)
+
+
+@pytest.mark.parametrize("width", [35, 224, 500, 4672, 40000])
+@pytest.mark.parametrize("cut", ["none", "k", "p"])
+def test_every_part_of_the_unit_interval(net, width, cut):
+    """One row drawn from many times, at evenly spread numbers."""
+    rng = np.random.default_rng(width)
+    rows = 2000 if width < 5000 else 300
+    one = some_logits(rng, 1, width, "f32")
+    u = ((np.arange(rows) + 0.5) / rows).astype(np.float32)
+    k = np.full(rows, 20, np.int32) if cut == "k" else None
+    p = np.full(rows, 0.9, np.float32) if cut == "p" else None
+    x = one.expand(rows, width)
+    assert x.stride(0) == 0
+    a = plain_adjusted(one.cpu().numpy(), None)
+    want, want_prob = plain_choice(np.broadcast_to(a, (rows, width)), None, k, p, u)
+    col, act, prob = call_choose(net, x, None, None, k, p, u)
+    assert np.array_equal(col, want) and np.array_equal(act, want)
+    assert (np.abs(prob - want_prob) <= want_prob * 2 * U + width * 2.0 ** -41).all()
+
+
+def test_long_lists(net):
+    """Histories and bias lists of thousands of entries, over slots and over actions, each action many times."""
+    rng = np.random.default_rng(12)
+    for rows, width, actions, slots in ((3, 224, 4672, True), (3, 600, 4672, True), (3, 300, 300, False), (2, 9001, 9001, False)):
+        x = some_logits(rng, rows, width, "f32")
+        rules = some_rules(rng, rows, width, actions, slots, history=20000, bias=3000)
+        check_adjust(net, x, rules, None)
