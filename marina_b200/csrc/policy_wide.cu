@@ -1041,9 +1041,13 @@ __global__ void __launch_bounds__(kMaxThreads) choose_wide_kernel(ChooseParams p
     const bool small = k > 0 && !p.in.rules.mask && border.few_k(mine, k);
     if (!small && k > 0) mem.left = compact(q, mem.x, weight, segment, mem.places, sh);
     if (small || border.few(k, top_p)) {
+      // The first block draws out of its own memory, but it may not leave while another still reads from
+      // it how many columns were gathered.
+      if (q.blocks > 1) cg::this_cluster().barrier_arrive();
       if (q.rank == 0)
         draw_few(p, row, mem.list, static_cast<int>(sh.listed[small ? 3 : 0]), k, top_p, sh.total_k, uniform, first, weight, sh);
-      return;  // the first block reads its own memory only
+      if (q.blocks > 1) cg::this_cluster().barrier_wait();
+      return;
     }
     last = border.find(k, top_p);
   }
