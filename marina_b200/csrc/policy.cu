@@ -49,11 +49,13 @@ __device__ __forceinline__ void flag_length(const SlotTableParams& p) {
 template <bool QUADS, int ROWS>
 __device__ __forceinline__ void fill_rows(const SlotTableParams& p, const int (&row)[ROWS], const int (&first)[ROWS],
                                           const int (&n)[ROWS], int lane) {
-  int listed[ROWS];  // <= 0 where the entries ended before, or there is no such row
+  // Columns are counted without a sign: a row may have 2^31 - 1 of them, and the last step goes past that.
+  const unsigned width = static_cast<unsigned>(p.width);
+  unsigned listed[ROWS];  // 0 where the entries ended before, or there is no such row
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) listed[i] = min(n[i], p.count - first[i]);
+  for (int i = 0; i < ROWS; ++i) listed[i] = static_cast<unsigned>(max(0, min(n[i], p.count - first[i])));
   if (QUADS) {
-    for (int s = 4 * lane; s < p.width; s += 128) {
+    for (unsigned s = 4 * lane; s < width; s += 128) {
       int4 v[ROWS];
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
@@ -72,7 +74,7 @@ __device__ __forceinline__ void fill_rows(const SlotTableParams& p, const int (&
         }
     }
   } else {
-    for (int s = lane; s < p.width; s += 32) {
+    for (unsigned s = lane; s < width; s += 32) {
       int v[ROWS];
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) v[i] = s < listed[i] ? __ldg(p.entries + first[i] + s) : -1;
@@ -84,7 +86,8 @@ __device__ __forceinline__ void fill_rows(const SlotTableParams& p, const int (&
   if (p.map) {
 #pragma unroll
     for (int i = 0; i < ROWS; ++i)
-      for (int s = lane; s < listed[i]; s += 32) p.map[first[i] + s] = row[i] * p.width + s;
+      for (unsigned s = lane; s < listed[i]; s += 32)
+        p.map[first[i] + s] = row[i] * p.width + static_cast<int>(s);
   }
 }
 
