@@ -243,44 +243,18 @@ __global__ void __launch_bounds__(kThreads) slot_fill_kernel(SlotTableParams p) 
 constexpr int kNarrowWarps = 4;
 constexpr int kCompared = 128;  // longest lists that are compared with a row's columns entry by entry
 
-// A warp's shared memory: a hash table from action to count (for slots; linear probing, at most half
-// full, so that a probe always ends), or a count for each column; then, for the choice, the columns
-// that are left.
+// A warp's shared memory: a table from action to count (for slots), or a count for each column; then, for
+// the choice, the columns that are left.
 template <int K>
 struct alignas(16) NarrowShared {
-  static constexpr int kEntries = 64 * K;  // twice the columns, a power of two
   union {
-    struct {
-      int keys[kEntries];
-      int counts[kEntries];
-    };
+    ActionCounts<64 * K> table;  // twice the columns, a power of two
     struct {
       uint64_t kept[32 * K];  // weight of the i-th column that is left, 0 once it is cut off
       float x[32 * K];
       int column[32 * K];
     };
   };
-
-  static __device__ __forceinline__ unsigned slot(int action) {
-    return (static_cast<unsigned>(action) * 2654435761u) >> 16 & (kEntries - 1);  // Knuth's multiplicative hash
-  }
-  __device__ __forceinline__ int insert(int action) {
-    unsigned h = slot(action);
-    for (;;) {
-      const int was = atomicCAS(&keys[h], -1, action);
-      if (was == -1 || was == action) return h;
-      h = (h + 1) & (kEntries - 1);
-    }
-  }
-  __device__ __forceinline__ int find(int action) const {
-    unsigned h = slot(action);
-    for (;;) {
-      const int k = keys[h];
-      if (k == action) return h;
-      if (k == -1) return -1;
-      h = (h + 1) & (kEntries - 1);
-    }
-  }
 };
 
 // Adjusted logits of a row. Returns the k whose columns are not all masked or empty, a bit each: lists of
@@ -372,23 +346,23 @@ __device__ __forceinline__ unsigned load_narrow(const LogitParams& p, int row, i
     if (SLOTS) {
 #pragma unroll
       for (int i = 0; i < K / 2; ++i) {
-        reinterpret_cast<int4*>(sh.keys)[32 * i + lane] = make_int4(-1, -1, -1, -1);
-        reinterpret_cast<int4*>(sh.counts)[32 * i + lane] = make_int4(0, 0, 0, 0);
+        reinterpret_cast<int4*>(sh.table.keys)[32 * i + lane] = make_int4(-1, -1, -1, -1);
+        reinterpret_cast<int4*>(sh.table.counts)[32 * i + lane] = make_int4(0, 0, 0, 0);
       }
     } else {
 #pragma unroll
-      for (int k = 0; k < K; ++k) sh.counts[32 * k + lane] = 0;
+      for (int k = 0; k < K; ++k) sh.table.counts[32 * k + lane] = 0;
     }
     __syncwarp();
     if (SLOTS) {
 #pragma unroll
       for (int k = 0; k < K; ++k)
-        if ((used >> k) & 1 && a[k] >= 0) at[k] = sh.insert(a[k]);
+        if ((used >> k) & 1 && a[k] >= 0) at[k] = sh.table.insert(a[k]);
       __syncwarp();
     }
     auto count = [&](int action) {
-      const int h = action < 0 ? -1 : SLOTS ? sh.find(action) : action < p.width ? action : -1;
-      if (h >= 0) atomicAdd(&sh.counts[h], 1);
+      const int h = action < 0 ? -1 : SLOTS ? sh.table.find(action) : action < p.width ? action : -1;
+      if (h >= 0) atomicAdd(&sh.table.counts[h], 1);
     };
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
@@ -398,7 +372,7 @@ __device__ __forceinline__ unsigned load_narrow(const LogitParams& p, int row, i
     if (pen.seen > 0) {
 #pragma unroll
       for (int k = 0; k < K; ++k)
-        if ((used >> k) & 1 && a[k] >= 0) v[k] = penalised(v[k], sh.counts[at[k]], pen);
+        if ((used >> k) & 1 && a[k] >= 0) v[k] = penalised(v[k], sh.table.counts[at[k]], pen);
     }
   }
   // Biases in the list's order: every lane looks one entry up, and the ones that name a column are
@@ -408,7 +382,7 @@ __device__ __forceinline__ unsigned load_narrow(const LogitParams& p, int row, i
       id = e0 + lane < biases ? ids[e0 + lane] : -1;
       value = e0 + lane < biases ? values[e0 + lane] : 0.f;
     }
-    const int h = id < 0 ? -1 : SLOTS ? sh.find(id) : id < p.width ? id : -1;
+    const int h = id < 0 ? -1 : SLOTS ? sh.table.find(id) : id < p.width ? id : -1;
     unsigned todo = __ballot_sync(~0u, h >= 0);
     while (todo) {
       const int j = __ffs(todo) - 1;

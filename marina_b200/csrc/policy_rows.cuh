@@ -42,6 +42,35 @@ __device__ __forceinline__ float penalised(float x, int count, const Penalties& 
   return __fsub_rn(__fsub_rn(x, __fmul_rn(p.frequency, static_cast<float>(count))), p.presence);
 }
 
+// Counts of actions in shared memory: a hash table of N places, a power of two, with linear probing, at
+// most half full, so that a probe always ends. Keys are -1 where a place is free.
+template <int N>
+struct ActionCounts {
+  int keys[N];
+  int counts[N];
+
+  static __device__ __forceinline__ unsigned slot(int action) {
+    return (static_cast<unsigned>(action) * 2654435761u) >> 16 & (N - 1);  // Knuth's multiplicative hash
+  }
+  __device__ __forceinline__ int insert(int action) {
+    unsigned h = slot(action);
+    for (;;) {
+      const int was = atomicCAS(&keys[h], -1, action);
+      if (was == -1 || was == action) return h;
+      h = (h + 1) & (N - 1);
+    }
+  }
+  __device__ __forceinline__ int find(int action) const {
+    unsigned h = slot(action);
+    for (;;) {
+      const int k = keys[h];
+      if (k == action) return h;
+      if (k == -1) return -1;
+      h = (h + 1) & (N - 1);
+    }
+  }
+};
+
 // Floats in an order that unsigned comparison keeps; the two zeros are one value.
 __device__ __forceinline__ uint32_t order_key(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);

@@ -3,6 +3,7 @@
 // exchange maxima, sums and histograms through distributed shared memory.
 #include <cooperative_groups.h>
 
+#include <algorithm>
 #include <type_traits>
 #include <utility>
 
@@ -137,10 +138,118 @@ __device__ __forceinline__ void store_span(T* to, int base, int n, const float (
   }
 }
 
+// Slots of a wide row, kTile of them at a time: a table of the actions that they name, which each entry of
+// the row's lists is looked up in once.
+constexpr int kTile = 2048;
+constexpr int kChunk = 1024;  // bias entries looked up at a time
+constexpr uint16_t kNoPlace = 0xffff;
+
+struct alignas(16) SlotTile {
+  ActionCounts<2 * kTile> table;
+  uint16_t at[kTile];  // each slot's place in the table, kNoPlace where it is masked or empty
+  int found[kChunk];   // each bias entry's place, -1 where no slot of the tile has its action
+  int found_in[kChunk / 32];  // of 32 entries each
+  struct {
+    int place;
+    float value;
+  } hits[kChunk];  // the entries that were found, in the list's order
+};
+static_assert(2 * kTile < kNoPlace && kChunk == 32 * 32, "places in 16 bits, a warp's lanes for the groups of a chunk");
+
+// Whether a row's lists are looked up in such a table. Shorter ones are compared with each slot entry by
+// entry, which leaves room for more blocks on a multiprocessor: at 192 entries, 4096 rows of 700 slots choose
+// in 178 us so and in 183 by the table (147 and 185 at 128 entries), 64 rows of 4096 adjust in 73 and 40.
+__host__ __device__ constexpr bool long_lists(int history, int biases) { return history + biases > 192; }
+
+// The adjusted logits of a block's slots into cells[0, q.n), where the row's lists are long. An entry costs
+// one look-up for each tile of slots, so that a row takes its columns / kTile passes over its lists, not
+// one for each column: 2 rows of 4096 slots with 65536 entries in both lists take 3.4 ms, compared column
+// by column 86 ms. Bound by latency: a segment has one thread to 32 slots. `action` gives the action of a slot, -1
+// where it is masked or empty.
+template <class T, class F>
+__device__ __forceinline__ void look_up_lists(const LogitParams& p, const Part& q, const Penalties& pen, const F& action,
+                                              float* cells, SlotTile& tile) {
+  const RuleParams& r = p.rules;
+  const int n = q.n, tid = threadIdx.x, threads = blockDim.x, row = q.row;
+  const int lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
+  const T* logits = static_cast<const T*>(p.logits) + row * p.stride + q.c0;
+  const int32_t* history = r.history + row * r.history_stride;
+  const int32_t* ids = r.bias_actions + row * r.bias_stride;
+  const float* values = r.bias_values + row * r.bias_stride;
+  for (int t0 = 0; t0 < n; t0 += kTile) {
+    const int m = min(kTile, n - t0);
+    __syncthreads();  // the tile before has been read
+    for (int i = tid; i < kTile / 2; i += threads) {
+      reinterpret_cast<int4*>(tile.table.keys)[i] = make_int4(-1, -1, -1, -1);
+      reinterpret_cast<int4*>(tile.table.counts)[i] = make_int4(0, 0, 0, 0);
+    }
+    __syncthreads();
+    for (int i = tid; i < m; i += threads) {
+      const int a = action(t0 + i);
+      tile.at[i] = a < 0 ? kNoPlace : static_cast<uint16_t>(tile.table.insert(a));
+    }
+    __syncthreads();
+    for (int h = tid; h < pen.seen; h += threads) {
+      const int a = history[h], place = a < 0 ? -1 : tile.table.find(a);
+      if (place >= 0) atomicAdd(&tile.table.counts[place], 1);
+    }
+    __syncthreads();
+    // Slot i is its thread's from here on.
+    for (int i = tid; i < m; i += threads)
+      cells[t0 + i] = tile.at[i] == kNoPlace ? -INFINITY
+                                             : penalised(as_float(logits[t0 + i]), tile.table.counts[tile.at[i]], pen);
+    for (int e0 = 0; e0 < r.bias_len; e0 += kChunk) {
+      for (int g = warp; g < kChunk / 32; g += warps) {
+        const int e = e0 + 32 * g + lane;
+        const int id = e < r.bias_len ? ids[e] : -1, place = id < 0 ? -1 : tile.table.find(id);
+        const unsigned here = __ballot_sync(~0u, place >= 0);
+        tile.found[32 * g + lane] = place;
+        if (lane == 0) tile.found_in[g] = __popc(here);
+      }
+      __syncthreads();
+      const int in_group = tile.found_in[lane];
+      const int hits = __reduce_add_sync(~0u, in_group);
+      for (int g = warp; g < kChunk / 32; g += warps) {
+        const int before = __reduce_add_sync(~0u, lane < g ? in_group : 0);
+        const int place = tile.found[32 * g + lane];
+        const unsigned here = __ballot_sync(~0u, place >= 0);
+        if (place >= 0)
+          tile.hits[before + __popc(here & ((1u << lane) - 1))] = {place, values[e0 + 32 * g + lane]};
+      }
+      __syncthreads();
+      if (hits) {
+        constexpr int kTogether = 4;  // slots of a thread: 3.4 ms in the case above, 5.9 ms one at a time
+        for (int i0 = tid; i0 < m; i0 += kTogether * threads) {
+          int place[kTogether];
+          float v[kTogether];
+#pragma unroll
+          for (int u = 0; u < kTogether; ++u) {
+            const int i = i0 + u * threads;
+            place[u] = i < m ? tile.at[i] : kNoPlace;
+            v[u] = i < m ? cells[t0 + i] : 0.f;
+          }
+          for (int h = 0; h < hits; ++h) {
+            const int at = tile.hits[h].place;
+            const float value = tile.hits[h].value;
+#pragma unroll
+            for (int u = 0; u < kTogether; ++u)
+              if (at == place[u]) v[u] = __fadd_rn(v[u], value);
+          }
+#pragma unroll
+          for (int u = 0; u < kTogether; ++u)
+            if (i0 + u * threads < m) cells[t0 + i0 + u * threads] = v[u];
+        }
+      }
+    }
+  }
+}
+
 // The adjusted logits of the block's columns, -inf behind the last. `cells` is shared memory for the
-// segment's columns, needed where the rows have a history or slots.
-template <class T, bool QUADS>
-__device__ __forceinline__ void load_part(const LogitParams& p, const Part& q, float* cells, float (&x)[kQuads][4]) {
+// segment's columns, needed where the rows have a history or slots; LOOK_UP: rows of slots that may have
+// long lists, with a SlotTile behind the cells.
+template <class T, bool QUADS, bool LOOK_UP>
+__device__ __forceinline__ void load_part(const LogitParams& p, const Part& q, int segment, float* cells,
+                                          float (&x)[kQuads][4]) {
   const RuleParams& r = p.rules;
   const int n = q.n, c0 = q.c0, tid = threadIdx.x, threads = blockDim.x, row = q.row;
   const T* logits = static_cast<const T*>(p.logits) + row * p.stride + c0;
@@ -149,21 +258,28 @@ __device__ __forceinline__ void load_part(const LogitParams& p, const Part& q, f
   const int32_t* history = r.history + row * r.history_stride;
   const int32_t* ids = r.bias_actions + row * r.bias_stride;
   const float* values = r.bias_values + row * r.bias_stride;
-  if (r.columns) {
-    // Slots of a wide row: each column counts its action in the history by itself.
+  if (LOOK_UP || r.columns) {
     const int32_t* columns = r.columns + row * r.columns_stride + c0;
-    for (int i = tid; i < n; i += threads) {
+    auto action = [&](int i) {  // -1 where the slot is masked or empty
       const int a = columns[i];
-      float v = -INFINITY;
       if (a >= r.actions && p.status) atomicCAS(p.status, 0, kErrBadAction);
-      if (a >= 0 && a < r.actions && (!mask || (mask[a >> 5] >> (a & 31)) & 1)) {
-        int count = 0;
-        for (int h = 0; h < pen.seen; ++h) count += history[h] == a;
-        v = penalised(as_float(logits[i]), count, pen);
-        for (int e = 0; e < r.bias_len; ++e)
-          if (ids[e] == a) v = __fadd_rn(v, values[e]);
+      return a >= 0 && a < r.actions && (!mask || (mask[a >> 5] >> (a & 31)) & 1) ? a : -1;
+    };
+    if (LOOK_UP && long_lists(pen.seen, r.bias_len)) {
+      look_up_lists<T>(p, q, pen, action, cells, *reinterpret_cast<SlotTile*>(cells + segment));
+    } else {
+      for (int i = tid; i < n; i += threads) {
+        const int a = action(i);
+        float v = -INFINITY;
+        if (a >= 0) {
+          int count = 0;
+          for (int h = 0; h < pen.seen; ++h) count += history[h] == a;
+          v = penalised(as_float(logits[i]), count, pen);
+          for (int e = 0; e < r.bias_len; ++e)
+            if (ids[e] == a) v = __fadd_rn(v, values[e]);
+        }
+        cells[i] = v;
       }
-      cells[i] = v;
     }
     __syncthreads();
 #pragma unroll
@@ -309,7 +425,7 @@ __device__ __forceinline__ int row_first(const Part& q, const float (&x)[kQuads]
 // names is looked up in shared memory between two barriers, and the row's other columns wait. 100 rows of
 // 100003 f16 under a mask: 12.4 us without lists, 36.5 us with histories of 4096 and 300 biases, which
 // every block of a row goes through.
-template <class T, bool QUADS>
+template <class T, bool QUADS, bool LOOK_UP>
 __global__ void __launch_bounds__(kMaxThreads) adjust_wide_kernel(AdjustParams p, int blocks, int segment) {
   extern __shared__ __align__(16) float cells[];
   __shared__ Exchange<uint32_t> ex_best;
@@ -319,7 +435,7 @@ __global__ void __launch_bounds__(kMaxThreads) adjust_wide_kernel(AdjustParams p
   grid_dep_launch();
   const Part q = my_part(blocks, segment, p.in.width);
   float x[kQuads][4];
-  load_part<T, QUADS>(p.in, q, cells, x);
+  load_part<T, QUADS, LOOK_UP>(p.in, q, segment, cells, x);
   if (p.out) {
     T* out = static_cast<T*>(p.out) + q.row * p.out_stride + q.c0;
 #pragma unroll
@@ -997,7 +1113,7 @@ __device__ __forceinline__ void draw_few(const ChooseParams& p, int row, const u
 // than the same work unrolled over registers, whose code does not stay in the cache. 2048 rows of 4672 f32
 // under a mask, top_k and top_p: 54 us; one row of 131072 bf16, top_k: 15.4 us; 64 rows of 150001 bf16 under
 // a mask, top_p alone: 118 us, for which one block of 608 threads fits a multiprocessor.
-template <class T, bool QUADS>
+template <class T, bool QUADS, bool LOOK_UP>
 __global__ void __launch_bounds__(kMaxThreads) choose_wide_kernel(ChooseParams p, int blocks, int segment) {
   extern __shared__ __align__(16) unsigned char dynamic[];
   __shared__ ChooseShared sh;
@@ -1012,7 +1128,7 @@ __global__ void __launch_bounds__(kMaxThreads) choose_wide_kernel(ChooseParams p
   const float top_p = p.top_p ? p.top_p[row] : 1.f;
   const float uniform = p.uniform ? p.uniform[row] : 0.f;
   float x[kQuads][4], mine;
-  load_part<T, QUADS>(p.in, q, mem.x, x);
+  load_part<T, QUADS, LOOK_UP>(p.in, q, segment, mem.x, x);
   const uint32_t best = row_best(q, x, sh.best, mine);
   const float m = key_value(best);
   const int first = best && best != ~0u && (t <= 0.f || !p.uniform) ? row_first<QUADS>(q, x, m, sh.first) : -1;
@@ -1128,11 +1244,18 @@ Shape wide_shape(const LogitParams& p) {
   return s;
 }
 
-// f(type, whether four columns are read at once) for the instantiations. They are where each row of
-// logits and of the outputs starts on a boundary of four elements.
+bool may_look_up(const LogitParams& p) { return p.rules.columns && long_lists(p.rules.history_len, p.rules.bias_len); }
+
+// f(type, whether four columns are read at once, whether lists may be looked up) for the instantiations.
+// Columns are read so where each row of logits and of the outputs starts on a boundary of four elements.
+// The look-up has kernels of its own, as its code costs the others registers (4096 rows of 4672, adjust:
+// 51.5 us with it and 48.7 without), and they read column by column, as they go through shared memory first.
 template <class F>
 cudaError_t with_wide(const LogitParams& p, bool quads, F&& f) {
-  return with_type(p.type, [&](auto v) { return quads ? f(v, std::true_type()) : f(v, std::false_type()); });
+  return with_type(p.type, [&](auto v) {
+    if (may_look_up(p)) return f(v, std::false_type(), std::true_type());
+    return quads ? f(v, std::true_type(), std::false_type()) : f(v, std::false_type(), std::false_type());
+  });
 }
 
 bool quad_rows(const void* base, int64_t stride, int size) {
@@ -1140,6 +1263,11 @@ bool quad_rows(const void* base, int64_t stride, int size) {
 }
 
 bool quad_rows(const LogitParams& p) { return quad_rows(p.logits, p.stride, p.type == LogitType::kF32 ? 4 : 2); }
+
+// Shared memory that load_part uses.
+size_t load_bytes(const LogitParams& p, int segment) {
+  return segment * sizeof(float) + (may_look_up(p) ? sizeof(SlotTile) : 0);
+}
 
 template <typename... Params, typename... Args>
 cudaError_t launch_rows(void (*kernel)(Params...), int rows, const Shape& shape, size_t smem, cudaStream_t stream,
@@ -1167,34 +1295,37 @@ cudaError_t launch_adjust_wide(const AdjustParams& p, cudaStream_t s) {
   const Shape shape = wide_shape(p.in);
   const bool quads = quad_rows(p.in) && (!p.out || quad_rows(p.out, p.out_stride, p.in.type == LogitType::kF32 ? 4 : 2)) &&
                      (!p.priors || quad_rows(p.priors, p.priors_stride, 4));
-  const size_t smem = p.in.rules.history || p.in.rules.columns ? shape.segment * sizeof(float) : 0;
-  return with_wide(p.in, quads, [&](auto v, auto q) {
-    return launch_rows(adjust_wide_kernel<decltype(v), q.value>, p.in.rows, shape, smem, s, p, shape.blocks,
+  const size_t smem = p.in.rules.history || p.in.rules.columns ? load_bytes(p.in, shape.segment) : 0;
+  return with_wide(p.in, quads, [&](auto v, auto q, auto look_up) {
+    return launch_rows(adjust_wide_kernel<decltype(v), q.value, look_up.value>, p.in.rows, shape, smem, s, p, shape.blocks,
                        shape.segment);
   });
 }
 
 cudaError_t launch_choose_wide(const ChooseParams& p, cudaStream_t s) {
   const Shape shape = wide_shape(p.in);
-  const size_t smem = ChooseMemory::bytes(shape.segment, shape.blocks, p.top_k || p.top_p);
-  return with_wide(p.in, quad_rows(p.in), [&](auto v, auto q) {
-    return launch_rows(choose_wide_kernel<decltype(v), q.value>, p.in.rows, shape, smem, s, p, shape.blocks,
+  const size_t smem = std::max(ChooseMemory::bytes(shape.segment, shape.blocks, p.top_k || p.top_p),
+                               load_bytes(p.in, shape.segment));
+  return with_wide(p.in, quad_rows(p.in), [&](auto v, auto q, auto look_up) {
+    return launch_rows(choose_wide_kernel<decltype(v), q.value, look_up.value>, p.in.rows, shape, smem, s, p, shape.blocks,
                        shape.segment);
   });
 }
 
 cudaError_t prepare_policy_wide() {
   for (LogitType t : {LogitType::kF32, LogitType::kF16, LogitType::kBf16})
-    for (bool quads : {false, true}) {
+    for (int form : {0, 1, 2}) {  // one column at a time, four, long lists of slots
       LogitParams in{};
-      in.type = t;
-      const cudaError_t e = with_wide(in, quads, [&](auto v, auto q) {
-        const cudaError_t r = cudaFuncSetAttribute(adjust_wide_kernel<decltype(v), q.value>,
+      const int32_t some = 0;
+      in.type = t, in.rules.columns = form == 2 ? &some : nullptr, in.rules.history_len = 1 << 20;
+      const cudaError_t e = with_wide(in, form == 1, [&](auto v, auto q, auto look_up) {
+        const cudaError_t r = cudaFuncSetAttribute(adjust_wide_kernel<decltype(v), q.value, look_up.value>,
                                                    cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   static_cast<int>(kMaxSegment * sizeof(float)));
+                                                   static_cast<int>(kMaxSegment * sizeof(float) + sizeof(SlotTile)));
         if (r != cudaSuccess) return r;
-        return cudaFuncSetAttribute(choose_wide_kernel<decltype(v), q.value>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    static_cast<int>(ChooseMemory::bytes(kMaxSegment, kMaxBlocks, true)));
+        return cudaFuncSetAttribute(choose_wide_kernel<decltype(v), q.value, look_up.value>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    static_cast<int>(std::max(ChooseMemory::bytes(kMaxSegment, kMaxBlocks, true),
+                                                              kMaxSegment * sizeof(float) + sizeof(SlotTile))));
       });
       if (e != cudaSuccess) return e;
     }

@@ -4,7 +4,7 @@ test_policy_gpu.py."""
 import numpy as np
 import pytest
 
-from tests.test_policy_gpu import clean_status, dev, here, net  # noqa: F401
+from tests.test_policy_gpu import Rules, check_adjust, check_choose, clean_status, dev, here, net, some_logits  # noqa: F401
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -32,3 +32,64 @@ def test_slot_rows_of_as_many_slots_as_there_may_be(net, rows, width):  # noqa: 
         assert int(row[n:].max()) == -1 == int(row[n:].min())
     assert np.array_equal(where.cpu().numpy(), np.concatenate([r * width + np.arange(n) for r in range(rows)]))
     assert net.status_word() == 0
+
+
+@pytest.mark.parametrize("width,history,bias", [(513, 1, 0), (640, 0, 1), (700, 190, 2), (700, 190, 3), (2047, 40, 1023), (2048, 2000, 1024),
+                                                (2049, 333, 1025), (6000, 5000, 3000), (20000, 700, 90),
+                                                (40000, 3000, 200)])
+def test_wide_slot_rows(net, width, history, bias):  # noqa: F811
+    """Slot rows above 512 columns, whose lists are looked up in 2048 of them at a time: actions that a row
+    names once, twice and in places far apart, biases whose sum depends on their order."""
+    rng = np.random.default_rng(width)
+    rows, actions = 3, 2 * width
+    columns = rng.integers(0, actions, (rows, width)).astype(np.int32)  # many of them twice
+    columns[0] = rng.permutation(actions)[:width]
+    columns[1, [0, width // 2, width - 1]] = 77
+    columns[2, rng.random(width) < 0.4] = -1
+    values = (rng.standard_normal((rows, bias)) * 10.0 ** rng.integers(-4, 5, (rows, bias))).astype(np.float32)
+    ids = rng.integers(-1, actions + 2, (rows, bias)).astype(np.int32)
+    ids[:, ::3] = 77
+    played = rng.integers(-2, actions + 2, (rows, history)).astype(np.int32)
+    played[:, ::2] = columns[:, :1]
+    rules = Rules(actions, columns, rng.random((rows, actions)) < 0.7, (ids, values) if bias else None,
+                  played if history else None, rng.integers(0, history + 1, rows).astype(np.int32) if history else None,
+                  (1 + rng.random(rows)).astype(np.float32), rng.random(rows).astype(np.float32),
+                  rng.random(rows).astype(np.float32) / 4)
+    rules.mask[:, 77] = True
+    for dtype in ("f32", "bf16"):
+        x = some_logits(rng, rows, width, dtype)
+        check_adjust(net, x, rules, None, dtype)
+        check_choose(net, x, rules, None, None, None, rng.random(rows).astype(np.float32), dtype)
+        check_choose(net, x, rules, None, np.full(rows, 9, np.int32), np.full(rows, 0.8, np.float32),
+                     rng.random(rows).astype(np.float32), dtype)
+    assert net.status_word() == 0
+
+
+def milliseconds(call):
+    call()
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    a.record()
+    call()
+    b.record()
+    torch.cuda.synchronize()
+    return a.elapsed_time(b)
+
+
+@pytest.mark.parametrize("rows,width,entries", [(2, 4096, 1 << 16)])
+def test_long_lists_over_wide_slot_rows(net, rows, width, entries):  # noqa: F811
+    """The lists are gone through once for a few thousand columns, not once for each column: 2^16 entries
+    of each list against 4096 columns are 5e8 comparisons a row, which took 86 ms; a look-up of each entry
+    takes 3 to 4. The bound lies between, a factor of four from either."""
+    rng = np.random.default_rng(1)
+    columns = np.stack([rng.permutation(2 * width)[:width] for _ in range(rows)]).astype(np.int32)
+    rules = Rules(2 * width, columns, None,
+                  (rng.integers(0, 2 * width, (rows, entries)).astype(np.int32),
+                   rng.standard_normal((rows, entries)).astype(np.float32)),
+                  rng.integers(0, 2 * width, (rows, entries)).astype(np.int32)).on_device()
+    x = dev(rng.standard_normal((rows, width)).astype(np.float32))
+    out = torch.empty_like(x)
+    column = torch.empty(rows, dtype=torch.int32, device="cuda:0")
+    adjust = lambda: net.adjust_logits(rows, width, x.data_ptr(), rules, out_ptr=out.data_ptr(), stream=here())
+    choose = lambda: net.choose_actions(rows, width, x.data_ptr(), rules, column.data_ptr(), stream=here())
+    took = milliseconds(adjust), milliseconds(choose)
+    assert max(took) < 20, took
