@@ -140,13 +140,16 @@ __device__ __forceinline__ double reciprocal(double v) {
 struct Weights {
   double m, steps;  // the largest logit; 32 log2(e) / t
   bool infinite;    // the largest logit is +inf: the columns that hold it share the row
-  float m32, inv_t32;
-  __device__ __forceinline__ Weights(float max, float t) : m(max), infinite(max == INFINITY), m32(max), inv_t32(1.f / t) {
+  float lowest;     // the smallest logit that may weigh anything
+  __device__ __forceinline__ Weights(float max, float t) : m(max), infinite(max == INFINITY) {
     steps = 46.166241308446828 * (t > 1e-30f && t < 1e30f ? reciprocal(t) : 1.0 / static_cast<double>(t));
+    // Below -41 ln 2 = -28.42 temperatures from the largest a weight rounds to 0. In f64 neither the product
+    // nor the difference leaves the range, at any temperature, and f32 logits are the whole test: those from
+    // the border rounded up on are those from the border on. -inf is never one of them.
+    lowest = infinite ? INFINITY : fmaxf(__double2float_ru(m - 28.5 * static_cast<double>(t)), -3.402823466e38f);
   }
-  // False only for logits that weigh 0: below -41 ln 2 = -28.42 the weight rounds to 0, and three
-  // roundings in f32 move -28.5 by less than 1e-5.
-  __device__ __forceinline__ bool maybe(float x) const { return !((x - m32) * inv_t32 < -28.5f) && x > -INFINITY; }
+  // False only for logits that weigh 0.
+  __device__ __forceinline__ bool maybe(float x) const { return x >= lowest; }
   __device__ __forceinline__ uint64_t operator()(float x) const {
     if (!maybe(x)) return 0;
     if (infinite) return x == INFINITY ? static_cast<uint64_t>(kWeightOne) : 0;

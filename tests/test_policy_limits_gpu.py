@@ -93,3 +93,35 @@ def test_long_lists_over_wide_slot_rows(net, rows, width, entries):  # noqa: F81
     choose = lambda: net.choose_actions(rows, width, x.data_ptr(), rules, column.data_ptr(), stream=here())
     took = milliseconds(adjust), milliseconds(choose)
     assert max(took) < 20, took
+
+
+F32 = np.finfo(np.float32)
+TINY = np.float32(2.0 ** -149)  # the smallest f32 above 0
+
+
+def far_rows(rng, width):
+    """Logits and temperatures whose difference leaves f32, or whose quotient needs a scale that does."""
+    z = rng.integers(0, 9, (9, width)).astype(np.float64)  # how many temperatures below the largest, about
+    z[:, rng.integers(0, width, 3)] = 0
+    t = np.array([1e38, 1e-40, TINY, F32.max, 1e-39, 2.0 ** 100, 2.0 ** 100 * 1.5, 2.0 ** -100, 2.0 ** -101], np.float32)
+    x = np.empty((9, width))
+    x[0] = 3e38 - z[0] * 0.75e38                 # the lowest 6e38 below the largest
+    x[1] = -z[1] * 1e-40
+    x[2] = (3 - z[2]) * TINY
+    x[3] = F32.max * (1 - z[3] / 4)              # two temperatures from end to end
+    x[4] = rng.standard_normal(width) * 1e-39
+    x[5:] = (z[5:] - 4) * t[5:, None]
+    return x.astype(np.float32), t
+
+
+@pytest.mark.parametrize("width", [40, 224, 500, 5000, 40000])
+def test_choice_of_logits_far_apart(net, width):  # noqa: F811
+    rng = np.random.default_rng(width + 2)
+    x, t = far_rows(rng, width)
+    rows = len(t)
+    rules = Rules(width, mask=rng.random(x.shape) < 0.5)
+    for u in (rng.random(rows).astype(np.float32), np.full(rows, 1 - 2.0 ** -24, np.float32), None):
+        for k in (None, np.full(rows, 5, np.int32), np.full(rows, width // 2, np.int32)):
+            for p in (None, np.full(rows, 0.9, np.float32)):
+                check_choose(net, dev(x), None, t, k, p, u)
+                check_choose(net, dev(x), rules, t, k, p, u)
