@@ -427,11 +427,11 @@ __global__ void __launch_bounds__(kNarrowWarps * 32) adjust_narrow_kernel(Adjust
   float* priors = p.priors + row * p.priors_stride;
   float sum = 0.f, inv;
   if (m > -INFINITY && m < INFINITY && t > 0.f) {
-    const float scale = exponent_scale(t);  // exp((v - m) / t)
+    const Exponential exponential(m, t);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       float e = 0.f;
-      if ((used >> k) & 1) e = power_of_two((v[k] - m) * scale);
+      if ((used >> k) & 1) e = exponential(v[k]);
       v[k] = e;
       sum += e;
     }

@@ -96,11 +96,21 @@ __device__ __forceinline__ float power_of_two(float v) {
   return r;
 }
 
-// log2(e) / t for t > 0, kept finite and above 0: with it (x - m) * scale is 0 for x = m and -inf for
-// x = -inf at every temperature, infinite ones and the smallest included.
-__device__ __forceinline__ float exponent_scale(float t) {
-  return fmaxf(fminf(1.44269504088896341f / t, 3.4e38f), 1.5e-45f);
-}
+// exp((x - m) / t) for a finite m and t > 0, as a power of two of (x - m) times log2(e) / t. Neither factor
+// may leave f32 where the product is of interest: above temperatures of 2^100 the logits are taken in units
+// of 2^64, below 2^-100 in units of 2^-100; the first moves the exponent by less than 2^-100, the second is
+// exact. In between a difference that overflows has a power of 0, and so has, below 2^-100, every logit
+// but the largest where that is 2^20 or more: the next one is 2^-4 or more away.
+struct Exponential {
+  float unit, m, scale;
+  __device__ __forceinline__ Exponential(float max, float t) {
+    unit = t > 0x1p100f ? 0x1p-64f : t < 0x1p-100f && fabsf(max) < 0x1p20f ? 0x1p100f : 1.f;
+    m = max * unit;
+    // 0 at a temperature of +inf, but 0 times -inf is not 0
+    scale = fmaxf(fminf(1.44269504088896341f / (t * unit), 3.4e38f), 1.5e-45f);
+  }
+  __device__ __forceinline__ float operator()(float x) const { return power_of_two(fmaf(x, unit, -m) * scale); }
+};
 
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);

@@ -449,12 +449,12 @@ __global__ void __launch_bounds__(kMaxThreads) adjust_wide_kernel(AdjustParams p
   float sum = 0.f, inv;
   auto total = [&]() { return row_reduce(q, sum, [](float a, float b) { return a + b; }, ex_sum); };
   if (best && best != ~0u && t > 0.f && m != INFINITY) {
-    const float scale = exponent_scale(t);  // exp((x - m) / t)
+    const Exponential exponential(m, t);
 #pragma unroll
     for (int k = 0; k < kQuads; ++k)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        x[k][j] = power_of_two((x[k][j] - m) * scale);
+        x[k][j] = exponential(x[k][j]);
         sum += x[k][j];
       }
     inv = 1.f / total();

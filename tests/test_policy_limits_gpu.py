@@ -101,17 +101,31 @@ TINY = np.float32(2.0 ** -149)  # the smallest f32 above 0
 
 def far_rows(rng, width):
     """Logits and temperatures whose difference leaves f32, or whose quotient needs a scale that does."""
-    z = rng.integers(0, 9, (9, width)).astype(np.float64)  # how many temperatures below the largest, about
+    z = rng.integers(0, 9, (12, width)).astype(np.float64)  # how many temperatures below the largest, about
     z[:, rng.integers(0, width, 3)] = 0
-    t = np.array([1e38, 1e-40, TINY, F32.max, 1e-39, 2.0 ** 100, 2.0 ** 100 * 1.5, 2.0 ** -100, 2.0 ** -101], np.float32)
-    x = np.empty((9, width))
+    t = np.array([1e38, 1e-40, TINY, F32.max, 1e-39, 2.0 ** 100, 2.0 ** 100 * 1.5, 2.0 ** -100, 2.0 ** -101, 1e-38, 1e-35, 1e-33],
+                 np.float32)
+    x = np.empty((12, width))
     x[0] = 3e38 - z[0] * 0.75e38                 # the lowest 6e38 below the largest
     x[1] = -z[1] * 1e-40
     x[2] = (3 - z[2]) * TINY
     x[3] = F32.max * (1 - z[3] / 4)              # two temperatures from end to end
     x[4] = rng.standard_normal(width) * 1e-39
-    x[5:] = (z[5:] - 4) * t[5:, None]
+    x[5:9] = (z[5:9] - 4) * t[5:9, None]
+    x[9] = 2.0 ** 20 - z[9] / 8                   # a step of f32 away: 2^120 temperatures
+    x[10] = -3e38 * (1 + z[10] / 64)
+    x[11] = 2.0 ** 20 - 2.0 ** -4 - z[11] / 16
     return x.astype(np.float32), t
+
+
+@pytest.mark.parametrize("width", [40, 224, 500, 5000, 40000])
+def test_priors_of_logits_far_apart(net, width):  # noqa: F811
+    x, t = far_rows(np.random.default_rng(width), width)
+    check_adjust(net, dev(x), None, t)
+    mask = np.random.default_rng(width + 1).random(x.shape) < 0.5
+    x[~mask] = -np.inf
+    check_adjust(net, dev(x), Rules(width, mask=mask), t)
+    check_adjust(net, dev(x), None, np.full(len(t), np.inf, np.float32))  # all that is left, in equal shares
 
 
 @pytest.mark.parametrize("width", [40, 224, 500, 5000, 40000])
