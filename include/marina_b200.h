@@ -261,8 +261,9 @@ MRN_API int mrn_evaluate_device_static(mrn_ctx* ctx, int n, const uint8_t* d_boa
  * Every pointer is to memory that the context's device can read and, for outputs, write, aligned to
  * its elements. The work is enqueued on `stream` without synchronising (a cudaStream_t of the
  * context's device; NULL = the context's own stream; the legacy default stream is the handle 1,
- * cudaStreamLegacy) and may be captured into a graph. The caller's current device is left as it
- * was. Nothing orders these calls with work on other streams, the context's passes included: that
+ * cudaStreamLegacy) and may be captured into a graph. With a stream of the caller's a call does not
+ * wait for a synchronous pass that another thread runs on the context; with NULL it waits until that
+ * call returns. The caller's current device is left as it was. Nothing orders these calls with work on other streams, the context's passes included: that
  * is the caller's, with events. Outputs must not overlap inputs or one another, except where it
  * says so. Numbers on the device cannot be refused by the call: what a bad one does is said with
  * the argument, and none of them makes a kernel read or write outside the buffers. Some set the

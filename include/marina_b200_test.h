@@ -58,6 +58,9 @@ MRN_TEST_API int mrn_test_layernorm(const void* x, const float* gamma, const flo
 MRN_TEST_API void* mrn_test_context(int device);
 MRN_TEST_API const char* mrn_test_context_error(void* ctx);
 MRN_TEST_API void mrn_test_context_free(void* ctx);
+/* Takes, on the calling thread, the lock that a synchronous pass on the context holds, and gives it back. */
+MRN_TEST_API void mrn_test_context_lock(void* ctx);
+MRN_TEST_API void mrn_test_context_unlock(void* ctx);
 
 MRN_TEST_API const char* mrn_test_last_error(void);
 

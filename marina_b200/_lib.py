@@ -44,7 +44,8 @@ EXPORTS = (
     "mrn_slot_table", "mrn_adjust_logits", "mrn_choose_actions", "mrn_evaluate_moves", "mrn_choose_moves",
 )
 TEST_EXPORTS = ("mrn_test_gemm", "mrn_test_gemm_wait_expiry", "mrn_test_attention", "mrn_test_layernorm",
-                "mrn_test_context", "mrn_test_context_error", "mrn_test_context_free", "mrn_test_last_error")
+                "mrn_test_context", "mrn_test_context_error", "mrn_test_context_free",
+                "mrn_test_context_lock", "mrn_test_context_unlock", "mrn_test_last_error")
 
 
 class MrnLinear(ctypes.Structure):
@@ -130,6 +131,8 @@ TEST_SIGNATURES = {
     "mrn_test_context": (c_void_p, [c_int]),
     "mrn_test_context_error": (c_char_p, [c_void_p]),
     "mrn_test_context_free": (None, [c_void_p]),
+    "mrn_test_context_lock": (None, [c_void_p]),
+    "mrn_test_context_unlock": (None, [c_void_p]),
     "mrn_test_last_error": (c_char_p, []),
     **{name: SIGNATURES[name] for name in ("mrn_slot_table", "mrn_adjust_logits", "mrn_choose_actions")},
 }

@@ -155,7 +155,11 @@ MRN_TEST_API void* mrn_test_context(int device) {
   return c;
 }
 
-MRN_TEST_API const char* mrn_test_context_error(void* ctx) { return static_cast<mrn_ctx*>(ctx)->last_error.c_str(); }
+MRN_TEST_API const char* mrn_test_context_error(void* ctx) { return static_cast<mrn_ctx*>(ctx)->last_error; }
+
+MRN_TEST_API void mrn_test_context_lock(void* ctx) { static_cast<mrn_ctx*>(ctx)->mu.lock(); }
+
+MRN_TEST_API void mrn_test_context_unlock(void* ctx) { static_cast<mrn_ctx*>(ctx)->mu.unlock(); }
 
 MRN_TEST_API void mrn_test_context_free(void* ctx) { delete static_cast<mrn_ctx*>(ctx); }
 

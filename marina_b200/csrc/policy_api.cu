@@ -121,6 +121,16 @@ struct DeviceScope {
   DeviceScope& operator=(const DeviceScope&) = delete;
 };
 
+// What a call reads of the context never changes, so that one on a stream of the caller's need not wait for a
+// synchronous pass, which holds the context's lock until it is done. The context's own stream may be in
+// capture under that lock (a batch size's first pass): a call on it has to wait.
+struct OwnStreamLock {
+  std::unique_lock<std::mutex> held;
+  OwnStreamLock(mrn_ctx* c, void* stream) : held(c->mu, std::defer_lock) {
+    if (!stream) held.lock();
+  }
+};
+
 cudaStream_t stream_of(const mrn_ctx* c, void* stream) { return stream ? static_cast<cudaStream_t>(stream) : c->stream; }
 
 }  // namespace
@@ -132,7 +142,7 @@ extern "C" {
 MRN_API int mrn_slot_table(mrn_ctx* c, int rows, int width, const int32_t* lengths, int count, const int32_t* entries,
                            int32_t* starts, int32_t* table, int32_t* map, void* stream) {
   if (!c) return MRN_ERR_ARGUMENT;
-  std::lock_guard<std::mutex> lock(c->mu);
+  const mrn::OwnStreamLock lock(c, stream);
   if (rows < 0 || width < 1 || count < 0)
     return c->fail(MRN_ERR_ARGUMENT, "slot table: rows %d, width %d, count %d", rows, width, count);
   if (static_cast<int64_t>(rows) * width > INT_MAX)
@@ -159,7 +169,7 @@ MRN_API int mrn_adjust_logits(mrn_ctx* c, int rows, int width, const void* logit
                               const mrn_rules* rules, const float* temperature, void* out, int64_t out_stride,
                               float* priors, int64_t priors_stride, void* stream) {
   if (!c) return MRN_ERR_ARGUMENT;
-  std::lock_guard<std::mutex> lock(c->mu);
+  const mrn::OwnStreamLock lock(c, stream);
   mrn::AdjustParams p{};
   const int rc = mrn::logit_params(c, rows, width, logits, type, stride, rules, temperature, &p.in);
   if (rc) return rc;
@@ -188,7 +198,7 @@ MRN_API int mrn_choose_actions(mrn_ctx* c, int rows, int width, const void* logi
                                const float* top_p, const float* uniform, int32_t* column, int32_t* action, float* prob,
                                void* stream) {
   if (!c) return MRN_ERR_ARGUMENT;
-  std::lock_guard<std::mutex> lock(c->mu);
+  const mrn::OwnStreamLock lock(c, stream);
   mrn::ChooseParams p{};
   const int rc = mrn::logit_params(c, rows, width, logits, type, stride, rules, temperature, &p.in);
   if (rc) return rc;

@@ -853,7 +853,7 @@ MRN_API int mrn_launches_per_forward(mrn_ctx* c, int n) {
 
 MRN_API const char* mrn_describe(mrn_ctx* c) { return c ? c->describe.c_str() : ""; }
 
-MRN_API const char* mrn_last_error(mrn_ctx* c) { return c ? c->last_error.c_str() : g_create_error.c_str(); }
+MRN_API const char* mrn_last_error(mrn_ctx* c) { return c ? c->last_error : g_create_error.c_str(); }
 
 MRN_API void mrn_destroy(mrn_ctx* c) { destroy(c); }
 

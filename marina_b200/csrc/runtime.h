@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 #include <stdarg.h>
 #include <stdio.h>
+#include <string.h>
 
 #include <map>
 #include <mutex>
@@ -128,7 +129,10 @@ struct mrn_ctx {
 
   std::map<int, mrn::Bucket> buckets;
   std::string describe;
-  std::string last_error;
+  // Written under its own lock, as the policy operators fail without `mu`. It never moves, so that a
+  // thread may read it while another call fails.
+  std::mutex error_mu;
+  char last_error[512] = {};
 
   int fail(int code, const char* fmt, ...) {
     char buf[512];
@@ -136,7 +140,8 @@ struct mrn_ctx {
     va_start(ap, fmt);
     vsnprintf(buf, sizeof(buf), fmt, ap);
     va_end(ap);
-    last_error = buf;
+    std::lock_guard<std::mutex> lock(error_mu);
+    memcpy(last_error, buf, strlen(buf) + 1);
     return code;
   }
 };
