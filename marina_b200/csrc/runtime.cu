@@ -502,7 +502,9 @@ bool is_pinned(const void* p) {
 
 int check_status(mrn_ctx* c, int word) {
   if (word == 0) return MRN_OK;
-  if (word == mrn::kErrBadAction) return c->fail(MRN_ERR_ACTION, "a legal slot held an action index >= %d", MRN_ACTIONS);
+  if (word == mrn::kErrBadAction)
+    return c->fail(MRN_ERR_ACTION, "a slot held an action index that is none: >= %d in a pass, >= rules.actions in a policy operator",
+                   MRN_ACTIONS);
   if (word == mrn::kErrBadLength)
     return c->fail(MRN_ERR_ARGUMENT, "a slot table's list length was outside [0, width], or its lists longer than the entries");
   return c->fail(MRN_ERR_DEVICE_FAULT, "device-side wait gave up in a GEMM (code %d)", word);

@@ -4,6 +4,8 @@ test_policy_gpu.py."""
 import numpy as np
 import pytest
 
+from marina_b200 import chess
+from marina_b200.network import NetworkError
 from tests.test_policy_gpu import Rules, check_adjust, check_choose, clean_status, dev, here, net, some_logits  # noqa: F401
 
 torch = pytest.importorskip("torch")
@@ -139,3 +141,18 @@ def test_choice_of_logits_far_apart(net, width):  # noqa: F811
             for p in (None, np.full(rows, 0.9, np.float32)):
                 check_choose(net, dev(x), None, t, k, p, u)
                 check_choose(net, dev(x), rules, t, k, p, u)
+
+
+def test_message_of_an_operators_bad_slot(net):  # noqa: F811
+    """The status word that an operator leaves fails the next synchronous call, whose message names the
+    operators' limit beside the pass's; the call after it is served."""
+    boards, legal, _, _ = chess.random_positions(3, 2, 0, 20)
+    want = net.evaluate_packed(boards, legal)
+    rules = Rules(70, np.array([[5, 70, 6, -1]], np.int32)).on_device()
+    x, out = torch.zeros((1, 4), device="cuda:0"), torch.zeros((1, 4), device="cuda:0")
+    net.adjust_logits(1, 4, x.data_ptr(), rules, out_ptr=out.data_ptr(), stream=here())
+    torch.cuda.synchronize()
+    with pytest.raises(NetworkError) as e:
+        net.evaluate_packed(boards, legal)
+    assert e.value.code == 7 and "rules.actions" in str(e.value)
+    assert all(np.array_equal(a, b) for a, b in zip(net.evaluate_packed(boards, legal), want))
