@@ -148,7 +148,8 @@ class MoveRules:
     * ``bias`` (actions [n or 1, k], values [n or 1, k]): added to the logits of those actions, -1
       where a list is shorter;
     * ``history`` [n or 1, h]: actions played before, -1 where a list is shorter, which ``repetition``,
-      ``presence`` and ``frequency`` (a number, or one per position) make less likely.
+      ``presence`` and ``frequency`` (a number, or one per position) make less likely. Without a history
+      there is nothing that they change.
     """
 
     def __init__(self, mask=None, bias=None, history=None, repetition=None, presence=None, frequency=None):
@@ -181,14 +182,15 @@ class MoveRules:
                 put("bias_actions", ids, "bias_stride")
                 put("bias_values", values)
                 parts["bias_len"] = ids.shape[1]
+        penalties = {name: _per_row(name, value, np.float32, n) for name, value in self.penalties.items()
+                     if value is not None}
         if self.history is not None:
             played = rows("history", self.history, np.int32)
             if played.shape[1]:
                 put("history", played, "history_stride")
                 parts["history_len"] = played.shape[1]
-            for name, value in self.penalties.items():
-                if value is not None:
-                    put(name, _per_row(name, value, np.float32, n))
+            for name, value in penalties.items():
+                put(name, value)
         rules = LogitRules(_lib.ACTIONS, **parts)
         rules.arrays = keep
         return rules

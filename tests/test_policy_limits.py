@@ -1,11 +1,12 @@
-"""The policy operators beside a pass on the same context, on a context without a device."""
+"""The policy operators beside a pass on the same context, on a context without a device, and the arguments of
+the calls on move lists."""
 
 import threading
 
 import pytest
 
 from marina_b200 import _lib
-from marina_b200.network import NetworkError
+from marina_b200.network import MoveRules, NetworkError
 from tests.test_policy_args import P, Q, net  # noqa: F401
 
 
@@ -56,3 +57,14 @@ def test_a_call_on_the_callers_stream_does_not_wait_for_a_pass(net, name):  # no
         for thread in threads:
             thread.join(20)
     assert got[0].code == 2
+
+
+@pytest.mark.parametrize("name", ["repetition", "presence", "frequency"])
+@pytest.mark.parametrize("history", [None, [[]], [[1, 2]]])
+def test_penalties_are_checked_with_and_without_a_history(name, history):
+    with pytest.raises(ValueError, match=name):
+        MoveRules(history=history, **{name: [1.0] * 5}).packed(3)
+    for value in (1.5, [1.0, 2.0, 3.0]):
+        packed = MoveRules(history=history, **{name: value}).packed(3)
+        assert packed.history_len == (2 if history == [[1, 2]] else 0)
+        assert bool(getattr(packed, name)) == (history is not None)
