@@ -1,12 +1,16 @@
 """The policy operators at the ends of what they accept, against the plain implementations of
 test_policy_gpu.py."""
 
+import threading
+
 import numpy as np
 import pytest
 
-from marina_b200 import chess
-from marina_b200.network import NetworkError
-from tests.test_policy_gpu import Rules, check_adjust, check_choose, clean_status, dev, here, net, some_logits  # noqa: F401
+from marina_b200 import chess, model, weights
+from marina_b200.network import B200Network, NetworkError
+from tests.test_policy_gpu import (TYPES, Rules, call_choose, check_adjust, check_choose, check_state, clean_status, dev,  # noqa: F401
+                                   here, make_state, net, plain_choice, plain_slot_table, some_logits, some_rules,
+                                   together)
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -156,3 +160,122 @@ def test_message_of_an_operators_bad_slot(net):  # noqa: F811
         net.evaluate_packed(boards, legal)
     assert e.value.code == 7 and "rules.actions" in str(e.value)
     assert all(np.array_equal(a, b) for a, b in zip(net.evaluate_packed(boards, legal), want))
+
+
+# Widths on both sides of a change of the kernel, of the columns that its threads hold, of the blocks of a row.
+BORDERS = [63, 64, 65, 256, 257, 511, 512, 513, 16383, 16384, 16385, 32768, 32769, 65536, 65537]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("width", BORDERS)
+def test_widths_where_the_kernels_change(net, width, dtype):  # noqa: F811
+    rng = np.random.default_rng(width)
+    rows = 3
+    x = some_logits(rng, rows, width, dtype)
+    t, u = (0.3 + rng.random(rows)).astype(np.float32), rng.random(rows).astype(np.float32)
+    k, p = np.array([3, width // 3, width - 1], np.int32), rng.random(rows).astype(np.float32)
+    for rules in (None, some_rules(rng, rows, width, width, False, history=700, bias=40),
+                  some_rules(rng, rows, width, 2 * width, True, history=30, bias=5)):
+        check_adjust(net, x, rules, t, dtype)
+        for kk, pp in ((None, None), (k, None), (None, p), (k, p)):
+            check_choose(net, x, rules, t, kk, pp, u, dtype)
+    # few distinct values: the cut-offs fall among equals, and lists of one value overflow
+    ties = torch.from_numpy(rng.integers(-1, 2, (rows, width)).astype(np.float32)).to("cuda:0").to(TYPES[dtype])
+    ties[0] = 1.0
+    for kk, pp in ((k, None), (None, p), (k, p)):
+        check_choose(net, ties, None, t, kk, pp, u, dtype)
+    assert net.status_word() == 0
+
+
+@pytest.mark.parametrize("cut", ["none", "k", "p"])
+@pytest.mark.parametrize("width", [50, 224, 512, 513, 4672, 16385, 40000])
+def test_numbers_outside_the_unit_interval(net, width, cut):  # noqa: F811
+    """From 1 on they draw the last column that is kept, below 0 and as NaN the first."""
+    rng = np.random.default_rng(width)
+    rows = 7
+    x = some_logits(rng, rows, width, "f32")
+    u = np.array([1, 2, np.inf, -1, -np.inf, np.nan, -0.0], np.float32)
+    k = np.full(rows, 20, np.int32) if cut == "k" else None
+    p = np.full(rows, 0.9, np.float32) if cut == "p" else None
+    want = plain_choice(x.cpu().numpy(), None, k, p, np.array([2, 2, 2, 0, 0, 0, 0], np.float32))[0]
+    assert np.array_equal(call_choose(net, x, None, None, k, p, u)[0], want)
+
+
+@pytest.mark.parametrize("shift,width,rows", [(1, 224, 100), (2, 8, 20000), (3, 512, 17000), (0, 500, 20000),
+                                              (0, 1000, 300), (1, 1001, 17000), (0, 30000, 5)])
+@pytest.mark.parametrize("with_map", [False, True])
+def test_slot_tables_anywhere(net, shift, width, rows, with_map):  # noqa: F811
+    """Tables that start at any element, of widths above a position's slots, with and without the map."""
+    rng = np.random.default_rng(width)
+    lengths = rng.integers(0, min(width, 40) + 1, rows).astype(np.int32)
+    lengths[rng.random(rows) < 0.02] = width
+    count = int(lengths.sum())
+    entries = rng.integers(0, 2**31 - 1, count).astype(np.int32)
+    whole = torch.full((shift + (rows + 1) * width,), -6, dtype=torch.int32, device="cuda:0")
+    starts = torch.full((rows + 2,), -5, dtype=torch.int32, device="cuda:0")
+    where = torch.full((count + 3,), -7, dtype=torch.int32, device="cuda:0")
+    le, en = dev(lengths), dev(entries)
+    net.slot_table(rows, width, le.data_ptr(), count, en.data_ptr(), starts.data_ptr(), whole[shift:].data_ptr(),
+                   where.data_ptr() if with_map else None, stream=here())
+    torch.cuda.synchronize()
+    want_starts, want, want_map = plain_slot_table(lengths, width, count, entries)
+    assert (whole[:shift] == -6).all() and (whole[shift + rows * width:] == -6).all()
+    assert np.array_equal(whole[shift: shift + rows * width].view(rows, width).cpu().numpy(), want)
+    assert np.array_equal(starts[:-1].cpu().numpy(), want_starts) and int(starts[-1]) == -5
+    assert np.array_equal(where[:count].cpu().numpy(), want_map if with_map else np.full(count, -7)) and (where[count:] == -7).all()
+    assert net.status_word() == 0
+
+
+def test_as_many_rows_as_there_may_be(net):  # noqa: F811
+    rows = 1 << 27
+    x = torch.full((1,), 2.0, device="cuda:0")
+    column, action = (torch.full((rows + 1,), -9, dtype=torch.int32, device="cuda:0") for _ in range(2))
+    prob = torch.full((rows + 1,), -9.0, device="cuda:0")
+    net.choose_actions(rows, 1, x.data_ptr(), None, column.data_ptr(), action.data_ptr(), prob.data_ptr(), stride=0,
+                       stream=here())
+    priors, out = torch.full((rows + 1,), -9.0, device="cuda:0"), torch.full((rows + 1,), -9.0, device="cuda:0")
+    net.adjust_logits(rows, 1, x.data_ptr(), None, out.data_ptr(), priors.data_ptr(), stride=0, stream=here())
+    torch.cuda.synchronize()
+    for got, want in ((column, 0), (action, 0), (prob, 1), (priors, 1), (out, 2)):
+        assert int((got[:-1] != want).sum()) == 0 and int(got[-1]) == -9
+
+
+def test_threads_beside_passes(cuda):
+    """Two threads run the operators on streams of theirs, a third on the context's own, while a fourth runs
+    passes on the same context, the first of each batch size with its capture."""
+    arch = model.Architecture(64, 1, 2, 128)
+    ctx = B200Network(arch, weights.random_init(arch), device=0, max_batch=64, precision="bf16")
+    boards, legal, _, _ = chess.random_positions(5, 64, 0, 40)
+    states = [make_state(20 + i, rows=300) for i in range(3)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    failures, results = [], {}
+
+    def run(call):
+        try:
+            call()
+        except Exception as e:  # handed to the test's thread
+            failures.append(e)
+
+    def operators(i):
+        for _ in range(100):
+            together(ctx, states[i], streams[i].cuda_stream if i < 2 else None)
+
+    def passes():
+        for n in (1, 2, 3, 5, 9, 17, 33, 64, 40, 20, 10):
+            results[n] = ctx.evaluate_packed(boards[:n], legal[:n])
+
+    threads = [threading.Thread(target=run, args=(lambda i=i: operators(i),)) for i in range(3)]
+    threads.append(threading.Thread(target=run, args=(passes,)))
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    assert not failures and not any(t.is_alive() for t in threads), failures
+    torch.cuda.synchronize()
+    for s in states:
+        check_state(s)
+    for n, got in results.items():
+        assert all(np.array_equal(a, b) for a, b in zip(got, ctx.evaluate_packed(boards[:n], legal[:n])))
+    assert ctx.status_word() == 0
+    ctx.close()
