@@ -91,8 +91,10 @@ __device__ __forceinline__ void fill_rows(const SlotTableParams& p, const int (&
   }
 }
 
-// Bound by HBM where there are many rows (262144 rows of 224: 63.5 us, 5.0 TB/s of the 6.57 measured for a
-// copy), by the launch where there are few (4096 rows: 4.0 us).
+// Bound by HBM where there are many rows (262144 rows of 224: 64.2 us, 4.9 TB/s of the 6.57 measured for a
+// copy), by the launch where there are few (4096 rows: 4.1 us). A warp takes a row whatever its width, so that
+// rows of other widths than a multiple of four store four bytes a lane, and rows of less than 128 slots leave lanes
+// idle.
 //
 // Few rows: one launch. Block b lays out the rows [b * per, (b + 1) * per), per <= 32, and finds where
 // they start by adding up every length before them: reading up to 64 KB that all blocks share in L2
@@ -238,8 +240,9 @@ __global__ void __launch_bounds__(kThreads) slot_fill_kernel(SlotTableParams p) 
 // 32 k + lane in v[k]: nothing but warp shuffles between its steps, and every global read of the row
 // in flight at once. K * 32 is the widest row of an instantiation.
 // Bound by the latency of a row's steps: 8192 rows of 224 slots without lists adjust in 5.9 us (5.2 TB/s,
-// inputs in L2), with 40 entries and 8 biases in 12.6 us, where the few rows with every slot filled come
-// last; the choice takes 28 us, most of it in f64 weights and in sorting those rows.
+// inputs in L2), with 40 entries and 8 biases in 12.8 us: rows of more than 64 moves pay for all 256 columns,
+// and the few with every slot filled come last. The choice takes 28 us; its first stall is for instructions
+// (four unrolled sorts, of which neighbouring warps run different ones), then come f64 weights.
 constexpr int kNarrowWarps = 4;
 constexpr int kCompared = 128;  // longest lists that are compared with a row's columns entry by entry
 
@@ -592,8 +595,11 @@ __global__ void __launch_bounds__(kNarrowWarps * 32) choose_narrow_kernel(Choose
 template <int N>
 using Int = std::integral_constant<int, N>;
 
-// Widest row of the one-warp kernels. 4096 rows of 512, adjust / choose, masked: 17.2 / 18.0 us by one
-// warp and 31.5 / 62.4 us by a block of 128 threads; unmasked: 16.2 / 58.7 and 36.0 / 76.7 us.
+// Widest row of the one-warp kernels, whatever the number of rows. By one warp and by a block of 128
+// threads, us without lists: 4096 rows of 512 adjust in 5.3 and 20.5, under a mask in 7.5 and 22.6, and
+// choose by top_p in 54.0 and 91.7, under a mask in 15.2 and 43.8. One row: 2.5 and 4.0, 3.5 and 4.1; 20.5
+// and 13.2, 5.9 and 9.4: only the choice from a few rows without a mask would be faster by a block (16 rows:
+// 21.1 and 20.0).
 constexpr int kNarrowWidth = 512;
 
 dim3 narrow_grid(int rows) { return dim3((rows + kNarrowWarps - 1) / kNarrowWarps); }

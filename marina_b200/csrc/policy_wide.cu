@@ -102,7 +102,7 @@ struct Quad {
   T v[4];
 };
 
-// f(i, j) for the columns i of span k inside the block's part.
+// The four columns that a lane holds of the span at `base`, -inf behind the n of the block's part.
 template <bool QUADS, class T>
 __device__ __forceinline__ void load_span(const T* from, int base, int n, float (&x)[4]) {
   if (QUADS && base + span_column<QUADS>(3) < n) {
@@ -420,11 +420,11 @@ __device__ __forceinline__ int row_first(const Part& q, const float (&x)[kQuads]
 }
 
 // Bound by HBM: a logit is read once, stays in a register through maximum, exponential and sum, and
-// leaves as its adjusted value and its prior. 4096 rows of 4672 f32 without lists take 37.9 us (6.1 TB/s of
-// the 6.57 measured for a copy), with a history of 40 entries and 16 biases 46.3 us (5.0 TB/s): what a list
+// leaves as its adjusted value and its prior. 4096 rows of 4672 f32 without lists take 38.4 us (6.0 TB/s of
+// the 6.57 measured for a copy), with a history of 40 entries and 16 biases 46.7 us (5.0 TB/s): what a list
 // names is looked up in shared memory between two barriers, and the row's other columns wait. 100 rows of
-// 100003 f16 under a mask: 12.4 us without lists, 36.5 us with histories of 4096 and 300 biases, which
-// every block of a row goes through.
+// 100003 f16 under a mask: 12.5 us without lists, 37.0 us with histories of 4096 and 300 biases: each of a
+// row's eight blocks goes through the whole history, and each of its warps through the whole bias list.
 template <class T, bool QUADS, bool LOOK_UP>
 __global__ void __launch_bounds__(kMaxThreads) adjust_wide_kernel(AdjustParams p, int blocks, int segment) {
   extern __shared__ __align__(16) float cells[];
@@ -495,8 +495,8 @@ __global__ void __launch_bounds__(kMaxThreads) adjust_wide_kernel(AdjustParams p
 // even the bin holds more than the list; and the draw goes over the whole row again.
 constexpr int kBins = 512;
 constexpr float kBinsPerUnit = 18.f;  // exp(-512 / 18) < 2^-41: what lies below weighs 0
-// Measured with and without the short way: 61.0 and 77.6 us for 2048 rows of 4672, 15.4 and 47.0 us for one
-// row of 131072.
+// Measured with and without the short way, for the few and for its list: 54.5 and 75.8 us for 2048 rows of
+// 4672, 15.8 and 46.8 us for one row of 131072, 114 and 127 us for 64 rows of 150001.
 constexpr int kFew = 256;
 
 __host__ __device__ constexpr int list_capacity(int segment) { return segment <= 8192 ? 1024 : 4096; }
@@ -1110,9 +1110,11 @@ __device__ __forceinline__ void draw_few(const ChooseParams& p, int row, const u
 
 // Bound by the latency of its steps, each a pass over shared memory between barriers, and by instruction
 // fetches (ncu: no_instruction and barrier are the first stalls): loops over shared memory are faster here
-// than the same work unrolled over registers, whose code does not stay in the cache. 2048 rows of 4672 f32
-// under a mask, top_k and top_p: 54 us; one row of 131072 bf16, top_k: 15.4 us; 64 rows of 150001 bf16 under
-// a mask, top_p alone: 118 us, for which one block of 608 threads fits a multiprocessor.
+// than the same work unrolled over registers, whose code does not stay in the cache. Blocks of up to 1024
+// threads leave it 64 registers, of which it spills 680 to 750 bytes a thread, blocks of 160 too. 2048 rows of
+// 4672 f32 under a mask, top_k and top_p: 54.8 us; one row of 131072 bf16, top_k and top_p: 15.5 us; 64 rows of
+// 150001 bf16 under a mask, top_p alone: 115 us, for which one block of 608 threads and 147 KB of shared memory fits a
+// multiprocessor, in 3.5 waves.
 template <class T, bool QUADS, bool LOOK_UP>
 __global__ void __launch_bounds__(kMaxThreads) choose_wide_kernel(ChooseParams p, int blocks, int segment) {
   extern __shared__ __align__(16) unsigned char dynamic[];
@@ -1152,8 +1154,8 @@ __global__ void __launch_bounds__(kMaxThreads) choose_wide_kernel(ChooseParams p
   if (k > 0 || top_p < 1.f) {
     Border border{q, mem, sh, weight, m, kBinsPerUnit / t};
     // Under a mask the threads' maxima say little about the few columns that are left: all are counted.
-    // Rows of 4672 of which one column in 16 is left: 54.1 us per 2048 so and 61.0 by the maxima; one row
-    // of 131072 without a mask: 19.2 and 15.4 us.
+    // Rows of 4672 of which one column in 16 is left: 54.5 us per 2048 so and 61.3 by the maxima; one row
+    // of 131072 without a mask: 19.8 and 15.8 us.
     const bool small = k > 0 && !p.in.rules.mask && border.few_k(mine, k);
     if (!small && k > 0) mem.left = compact(q, mem.x, weight, segment, mem.places, sh);
     if (small || border.few(k, top_p)) {
@@ -1227,11 +1229,22 @@ struct Shape {
   int blocks, segment, threads;
 };
 
-// Blocks per row, and threads: as many as hold the segment. A row of up to 16384 columns is one block's
-// even where that leaves multiprocessors idle, as what blocks exchange costs more than they save (us,
-// adjust / choose, 1 row of 4672: 5.2 / 8.8 by one block, 6.3 / 10.2 by two; 512 rows of 16000: 22.2 / 44.9
-// and 24.4 / 41.8). Above, blocks take 8192 columns each (128 rows of 60000: 24.6 / 38.0 by eight blocks,
-// 25.5 / 49.9 by four), or an eighth of the row.
+// Blocks per row, and threads: as many as hold the segment. A row of up to 16384 columns is one block's,
+// wider ones have four or eight blocks of 4097 to 8192 columns, or eight of up to 32768. The rule looks at
+// the width alone and is one for both operators, which does not suit all of them (us by 1 / 2 / 4 / 8 blocks, logits
+// without lists, the choice by top_p alone):
+//                     adjust                      choose
+//   1 x 4672           3.6 / 5.2 / 5.5 / 5.9      32.4 / 24.1 / 20.4 / 18.5
+//   512 x 4672         5.7 / 8.2 / 14.9 / 29.7    40.3 / 56.5 / 70.7 / 101.0
+//   1 x 16000          5.8 / 5.7 / 5.5 / 5.9      36.8 / 40.5 / 37.0 / 25.2
+//   512 x 16000       16.6 / 20.0 / 20.2 / 31.9  116.3 / 103.8 / 143.9 / 164.9
+//   1 x 60000            - / 10.7 / 7.6 / 6.4        - / 44.2 / 45.0 / 41.2
+//   128 x 60000          - / 22.8 / 22.4 / 21.7      - / 106.1 / 149.0 / 116.7
+//   1 x 100000           -  /  -  / 9.9 / 7.7        -  /  -  / 48.4 / 43.5
+//   128 x 100000         -  /  -  / 44.9 / 44.3      -  /  -  / 191.4 / 328.8
+// Adjust is within 7 % of its best everywhere. The choice is not: a single row of one block would be faster on
+// eight, and many rows of 100000 on four, as a segment above 8192 columns takes a list of 32 KB
+// (list_capacity) and leaves room for one block on a multiprocessor.
 Shape wide_shape(const LogitParams& p) {
   const int width = p.width;
   int blocks = 1;
