@@ -8,9 +8,9 @@ import pytest
 
 from marina_b200 import chess, model, weights
 from marina_b200.network import B200Network, NetworkError
-from tests.test_policy_gpu import (TYPES, Rules, call_choose, check_adjust, check_choose, check_state, clean_status, dev,  # noqa: F401
-                                   here, make_state, net, plain_choice, plain_slot_table, some_logits, some_rules,
-                                   together)
+from tests.test_policy_gpu import (TYPES, Rules, call_choose, check_adjust, check_choose, check_priors, check_state,  # noqa: F401
+                                   clean_status, dev, here, make_state, net, plain_adjusted, plain_choice,
+                                   plain_slot_table, some_logits, some_rules, together)
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -42,7 +42,7 @@ def test_slot_rows_of_as_many_slots_as_there_may_be(net, rows, width):  # noqa: 
 
 @pytest.mark.parametrize("width,history,bias", [(513, 1, 0), (640, 0, 1), (700, 190, 2), (700, 190, 3), (2047, 40, 1023), (2048, 2000, 1024),
                                                 (2049, 333, 1025), (6000, 5000, 3000), (20000, 700, 90),
-                                                (40000, 3000, 200)])
+                                                (40000, 3000, 200), (262144, 900, 60)])
 def test_wide_slot_rows(net, width, history, bias):  # noqa: F811
     """Slot rows above 512 columns, whose lists are looked up in 2048 of them at a time: actions that a row
     names once, twice and in places far apart, biases whose sum depends on their order."""
@@ -279,3 +279,46 @@ def test_threads_beside_passes(cuda):
         assert all(np.array_equal(a, b) for a, b in zip(got, ctx.evaluate_packed(boards[:n], legal[:n])))
     assert ctx.status_word() == 0
     ctx.close()
+
+
+def test_large_calls_in_a_graph(net):  # noqa: F811
+    """A slot table in three launches, rows of several blocks and long lists over wide slot rows, captured once
+    and replayed with other inputs in the same buffers."""
+    rows, width, tall = 4, 20000, 20000
+    rng = np.random.default_rng(4)
+    lengths, entries = torch.zeros(tall, dtype=torch.int32, device="cuda:0"), torch.zeros(9 * tall, dtype=torch.int32, device="cuda:0")
+    starts, table = torch.zeros(tall + 1, dtype=torch.int32, device="cuda:0"), torch.zeros((tall, 9), dtype=torch.int32, device="cuda:0")
+    where = torch.zeros(9 * tall, dtype=torch.int32, device="cuda:0")
+    rules = some_rules(rng, rows, width, 2 * width, True, history=300, bias=50)
+    r = rules.on_device()
+    x, out, priors = (torch.zeros((rows, width), device="cuda:0") for _ in range(3))
+    u, p = torch.zeros(rows, device="cuda:0"), torch.full((rows,), 0.8, device="cuda:0")
+    column = torch.zeros(rows, dtype=torch.int32, device="cuda:0")
+
+    def calls():
+        s = torch.cuda.current_stream().cuda_stream
+        net.slot_table(tall, 9, lengths.data_ptr(), 9 * tall, entries.data_ptr(), starts.data_ptr(), table.data_ptr(),
+                       where.data_ptr(), stream=s)
+        net.adjust_logits(rows, width, x.data_ptr(), r, out_ptr=out.data_ptr(), priors_ptr=priors.data_ptr(), stream=s)
+        net.choose_actions(rows, width, x.data_ptr(), r, column.data_ptr(), top_p_ptr=p.data_ptr(), uniform_ptr=u.data_ptr(),
+                           stream=s)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls()
+    for _ in range(3):
+        n = rng.integers(0, 10, tall).astype(np.int32)
+        e = rng.integers(0, 99, 9 * tall).astype(np.int32)
+        lengths.copy_(dev(n)), entries.copy_(dev(e)), where.fill_(-7)
+        x.copy_(some_logits(rng, rows, width, "f32")), u.copy_(torch.rand(rows, device="cuda:0"))
+        torch.cuda.synchronize()
+        graph.replay()
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, want in zip((starts, table, where), plain_slot_table(n, 9, 9 * tall, e)):
+            assert np.array_equal(got.cpu().numpy(), want)
+        a = plain_adjusted(x.cpu().numpy(), rules)
+        assert np.array_equal(out.cpu().numpy(), a)
+        check_priors(priors.cpu().numpy(), a, None)
+        assert np.array_equal(column.cpu().numpy(), plain_choice(a, None, None, p.cpu().numpy(), u.cpu().numpy())[0])
+    assert net.status_word() == 0
