@@ -13,7 +13,8 @@
  *   - The caller owns every host buffer it passes; the library owns the device memory,
  *     pinned staging buffers, streams and CUDA graphs of a context.
  *   - One context per GPU. Calls on one context may come from any thread (the device is made
- *     current on each call); the library serialises them, and the GPU work of each pass waits
+ *     current on each call); the library serialises them (but for the policy operators on a
+ *     caller's stream, which wait for no other call), and the GPU work of each pass waits
  *     for the context's previous pass even when the two were enqueued on different streams
  *     (except while the caller's stream is being captured into a graph, where ordering the
  *     captured work is the caller's).
